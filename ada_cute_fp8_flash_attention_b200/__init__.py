@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import importlib.util
 import sys
+from typing import Any, NamedTuple
 
 from . import _build
 
@@ -29,6 +30,12 @@ __all__ = [
     "flash_attn_fp8_backward",
     "lse_merge",
     "quantize_e4m3",
+    "KVCacheFP8",
+    "kv_cache_alloc",
+    "kv_cache_write",
+    "kv_cache_read",
+    "flash_attn_fp8_decode",
+    "flash_attn_fp8_shared_prefix",
     "launch_count",
 ]
 
@@ -131,6 +138,114 @@ def lse_merge(outs, lses):
 def quantize_e4m3(x, scale=1.0, transpose_last2=False):
     """fp16/bf16 -> e4m3 (RNE, saturating at +-448), optionally transposing the last 2 dims."""
     return _C.quantize_e4m3(x, scale, transpose_last2)
+
+
+class KVCacheFP8(NamedTuple):
+    """A paged e4m3 key/value cache: the tensors and nothing else.
+
+    ``k``, ``v``: float8_e4m3fn (pages, H_kv, page_size, D), unit last stride, the
+    other strides multiples of 16 (a (pages, page_size, H_kv, D) tensor is passed as
+    its ``transpose(1, 2)``); ``k_exp``, ``v_exp``: uint8 (pages, H_kv, page_size),
+    unit last stride. The row of a token and head has the values
+    ``code * 2**(exp - 127)``; 255 marks a row that held an infinity or a NaN and
+    reads as NaN. page_size is 16, 32, 64 or a multiple of 128, D 64 or 128.
+    """
+    k: Any
+    v: Any
+    k_exp: Any
+    v_exp: Any
+
+
+def kv_cache_alloc(num_pages, heads_kv, page_size, head_dim, device="cuda"):
+    """A new ``KVCacheFP8`` on ``device``: zero codes, unit exponents."""
+    import torch
+    shape = (num_pages, heads_kv, page_size)
+
+    def codes():
+        return torch.zeros(*shape, head_dim, dtype=torch.uint8, device=device).view(
+            torch.float8_e4m3fn)
+
+    def exps():
+        return torch.full(shape, 127, dtype=torch.uint8, device=device)
+    return KVCacheFP8(codes(), codes(), exps(), exps())
+
+
+def kv_cache_write(cache, k, v, page_table, seqlens, cu_seqlens=None, status=None):
+    """Quantise new tokens' K and V into a paged e4m3 cache (in place).
+
+    ``page_table`` int32 (batch, max_pages): token t of sequence b lies in slot
+    t % page_size of page ``page_table[b, t // page_size]``. ``seqlens`` int32
+    (batch): tokens each sequence holds with the new ones, as
+    ``flash_attn_fp8_decode`` takes it; the new tokens are its last. ``k``, ``v``
+    (fp16 or bf16): (batch, H_kv, S_new, D), or packed (tokens, H_kv, D) with
+    ``cu_seqlens`` int32 (batch + 1); rows outside cu_seqlens[0]..cu_seqlens[-1]
+    are ignored. Every row gets the least power of two that brings its largest
+    magnitude to 448 or less (2**-63 at least) and e4m3 codes rounded once to
+    nearest even.
+
+    Tables and lengths are never read on the host. What does not fit is not
+    written and ORs a bit into ``status`` (optional int32 device tensor): 4 = a
+    sequence longer than its table row, or shorter than its new tokens; 8 = a page
+    id outside the cache. No two tokens of a call may share a slot.
+    """
+    _C.kv_cache_write(cache[0], cache[1], cache[2], cache[3], k, v, page_table, seqlens,
+                      cu_seqlens, status)
+
+
+def kv_cache_read(cache, page_table, seqlens, cu_seqlens, total, dtype="fp16", out=None,
+                  status=None):
+    """Each sequence's last tokens read back from a paged e4m3 cache: (k, v).
+
+    With ``cu_seqlens`` int32 (batch + 1) the last cu_seqlens[b + 1] - cu_seqlens[b]
+    tokens of sequence b, packed (total, H_kv, D); with ``cu_seqlens=None`` the last
+    ``total`` tokens of each, (batch, H_kv, total, D). ``dtype`` "fp16" or "bf16":
+    ``code * 2**(exp - 127)`` rounded once, saturating. ``out``: (k, v) tensors to
+    write to; rows outside cu_seqlens[0]..cu_seqlens[-1] and refused sequences
+    (``status`` bit 4) are left as they were there (and undefined without ``out``),
+    tokens on a page id outside the cache (bit 8) are NaN. ``total`` is a host
+    number: nothing is read from the device.
+    """
+    ok, ov = (None, None) if out is None else out
+    k, v = _C.kv_cache_read(cache[0], cache[1], cache[2], cache[3], page_table, seqlens,
+                            cu_seqlens, total, dtype, ok, ov, status)
+    return k, v
+
+
+def flash_attn_fp8_decode(q, cache, page_table, seqlens, softmax_scale=None, return_lse=False,
+                          out=None, status=None):
+    """Attention of each sequence's last tokens over a paged e4m3 cache.
+
+    ``q`` fp16 or bf16 (B, H, S_q, D), S_q = 1 for a decoding step, more for drafted
+    tokens or a chunk of a prompt; ``cache``, ``page_table`` (B, max_pages) and
+    ``seqlens`` (B) as ``kv_cache_write`` left them, the S_q tokens included: query i
+    of sequence b has position seqlens[b] - S_q + i and sees the keys up to it. H is a
+    multiple of the cache's H_kv. Returns ``out`` (q's shape and dtype) or
+    ``(out, lse)``, lse fp32 (B, H, S_q), natural log; queries that see no key give 0
+    and -inf. Lengths stay on the device and any mixture of them shares the GPU
+    evenly. ``status`` (optional int32 device tensor) bits: 4 = a sequence whose
+    length does not fit its table row, left unwritten; 8 = a page id outside the
+    cache, its sequence's queries that see it are NaN; 1 = a wait inside the kernel
+    gave up.
+    """
+    res = _C.flash_attn_fp8_decode(q, cache[0], cache[1], cache[2], cache[3], page_table, seqlens,
+                                   0, softmax_scale, return_lse, out, status)
+    return (res[0], res[1]) if return_lse else res[0]
+
+
+def flash_attn_fp8_shared_prefix(q, cache, page_table, seqlens, prefix_len, softmax_scale=None,
+                                 return_lse=False, out=None, status=None):
+    """``flash_attn_fp8_decode`` for a batch whose sequences begin with the same tokens.
+
+    The first ``prefix_len`` tokens (a host number, any value a table row can hold)
+    are read once for the whole batch, from the pages of ``page_table``'s row 0, and
+    all the batch's queries meet them together; the other rows' entries for whole
+    prefix pages are not read. The result is that of ``flash_attn_fp8_decode`` up to
+    the order of its sums, given that every row's first prefix_len tokens hold what
+    row 0's hold. Sequences shorter than the prefix see their own length of it.
+    """
+    res = _C.flash_attn_fp8_decode(q, cache[0], cache[1], cache[2], cache[3], page_table, seqlens,
+                                   int(prefix_len), softmax_scale, return_lse, out, status)
+    return (res[0], res[1]) if return_lse else res[0]
 
 
 def launch_count():

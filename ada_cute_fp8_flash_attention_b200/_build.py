@@ -32,8 +32,8 @@ NVCC_FLAGS = [
     "-Xptxas", "-v",
 ]
 
-CUDA_SOURCES = ["fa8_api.cu", "fa8_aux.cu", "fa8_bwd.cu"]
-CUDA_HEADERS = ["fa8_fwd_kernel.cuh", "fa8_softmax.cuh", "sm100_ptx.cuh"]
+CUDA_SOURCES = ["fa8_api.cu", "fa8_aux.cu", "fa8_bwd.cu", "fa8_kv.cu", "fa8_decode.cu"]
+CUDA_HEADERS = ["fa8_fwd_kernel.cuh", "fa8_softmax.cuh", "fa8_kv.cuh", "sm100_ptx.cuh"]
 
 
 def _nvcc() -> str:

@@ -22,6 +22,8 @@ FA8_V_BHDS = 0
 FA8_V_BHSD = 1
 FA8_OUT_F16 = 0
 FA8_OUT_E4M3 = 1
+FA8_DT_F16 = 0
+FA8_DT_BF16 = 1
 
 # Every symbol include/fa8.h declares.
 EXPORTED = [
@@ -35,6 +37,12 @@ EXPORTED = [
     "fa8_bwd_params_init",
     "fa8_bwd_workspace_size",
     "fa8_bwd",
+    "fa8_kv_cache_init",
+    "fa8_kv_write",
+    "fa8_kv_read",
+    "fa8_decode_params_init",
+    "fa8_decode_workspace_size",
+    "fa8_decode",
     "fa8_status_string",
     "fa8_last_error_message",
     "fa8_launch_count",
@@ -83,6 +91,44 @@ class Fa8BwdParams(C.Structure):
     ]
 
 
+class Fa8KvCache(C.Structure):
+    """Mirror of ``struct fa8_kv_cache``."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+        ("num_pages", C.c_int64), ("heads_kv", C.c_int64), ("page_size", C.c_int64),
+        ("head_dim", C.c_int64),
+        ("k_stride_p", C.c_int64), ("k_stride_h", C.c_int64), ("k_stride_s", C.c_int64),
+        ("v_stride_p", C.c_int64), ("v_stride_h", C.c_int64), ("v_stride_s", C.c_int64),
+        ("k_exp_stride_p", C.c_int64), ("k_exp_stride_h", C.c_int64),
+        ("v_exp_stride_p", C.c_int64), ("v_exp_stride_h", C.c_int64),
+        ("batch", C.c_int64), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("max_pages", C.c_int64), ("seqlens", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class Fa8KvCopyParams(C.Structure):
+    """Mirror of ``struct fa8_kv_copy_params``."""
+    _fields_ = [
+        ("cache", Fa8KvCache), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("cu_seqlens", C.c_void_p), ("tokens", C.c_int64),
+        ("k_stride_b", C.c_int64), ("k_stride_h", C.c_int64), ("k_stride_s", C.c_int64),
+        ("v_stride_b", C.c_int64), ("v_stride_h", C.c_int64), ("v_stride_s", C.c_int64),
+        ("dtype", C.c_int32), ("reserved0", C.c_int32),
+    ]
+
+
+class Fa8DecodeParams(C.Structure):
+    """Mirror of ``struct fa8_decode_params``."""
+    _fields_ = [
+        ("cache", Fa8KvCache), ("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("heads", C.c_int64), ("seqlen_q", C.c_int64),
+        ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64), ("q_stride_s", C.c_int64),
+        ("o_stride_b", C.c_int64), ("o_stride_h", C.c_int64), ("o_stride_s", C.c_int64),
+        ("prefix_len", C.c_int64), ("softmax_scale", C.c_float), ("dtype", C.c_int32),
+        ("wait_timeout_cycles", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -115,6 +161,18 @@ def lib(path: Path | None = None) -> C.CDLL:
         L.fa8_bwd_workspace_size.restype = C.c_int64
         L.fa8_bwd.argtypes = [C.POINTER(Fa8BwdParams), C.c_void_p, C.c_int64, C.c_void_p]
         L.fa8_bwd.restype = C.c_int
+        L.fa8_kv_cache_init.argtypes = [C.POINTER(Fa8KvCache)] + [C.c_int64] * 6
+        L.fa8_kv_cache_init.restype = None
+        for name in ("fa8_kv_write", "fa8_kv_read"):
+            fn = getattr(L, name)
+            fn.argtypes = [C.POINTER(Fa8KvCopyParams), C.c_void_p]
+            fn.restype = C.c_int
+        L.fa8_decode_params_init.argtypes = [C.POINTER(Fa8DecodeParams)] + [C.c_int64] * 8
+        L.fa8_decode_params_init.restype = None
+        L.fa8_decode_workspace_size.argtypes = [C.POINTER(Fa8DecodeParams)]
+        L.fa8_decode_workspace_size.restype = C.c_int64
+        L.fa8_decode.argtypes = [C.POINTER(Fa8DecodeParams), C.c_void_p, C.c_int64, C.c_void_p]
+        L.fa8_decode.restype = C.c_int
         L.fa8_status_string.argtypes = [C.c_int]
         L.fa8_status_string.restype = C.c_char_p
         L.fa8_last_error_message.argtypes = []
@@ -182,3 +240,37 @@ def bwd_workspace_size(p: Fa8BwdParams) -> int:
 
 def bwd(p: Fa8BwdParams, workspace: int, workspace_bytes: int, stream: int = 0) -> int:
     return lib().fa8_bwd(C.byref(p), C.c_void_p(workspace), workspace_bytes, C.c_void_p(stream))
+
+
+def kv_copy_params(num_pages, heads_kv, page_size, head_dim, batch, max_pages) -> Fa8KvCopyParams:
+    """A zeroed copy call whose cache part is contiguous."""
+    p = Fa8KvCopyParams()
+    lib().fa8_kv_cache_init(C.byref(p.cache), num_pages, heads_kv, page_size, head_dim, batch,
+                            max_pages)
+    return p
+
+
+def kv_write(p: Fa8KvCopyParams, stream: int = 0) -> int:
+    return lib().fa8_kv_write(C.byref(p), C.c_void_p(stream))
+
+
+def kv_read(p: Fa8KvCopyParams, stream: int = 0) -> int:
+    return lib().fa8_kv_read(C.byref(p), C.c_void_p(stream))
+
+
+def decode_params(num_pages, heads_kv, page_size, head_dim, batch, max_pages, heads,
+                  seqlen_q) -> Fa8DecodeParams:
+    p = Fa8DecodeParams()
+    lib().fa8_decode_params_init(C.byref(p), num_pages, heads_kv, page_size, head_dim, batch,
+                                 max_pages, heads, seqlen_q)
+    return p
+
+
+def decode_workspace_size(p: Fa8DecodeParams) -> int:
+    """Device workspace bytes fa8_decode needs for these parameters (-1: invalid)."""
+    return int(lib().fa8_decode_workspace_size(C.byref(p)))
+
+
+def decode(p: Fa8DecodeParams, workspace: int, workspace_bytes: int, stream: int = 0) -> int:
+    return lib().fa8_decode(C.byref(p), C.c_void_p(workspace), workspace_bytes,
+                            C.c_void_p(stream))

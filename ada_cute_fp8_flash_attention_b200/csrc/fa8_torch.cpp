@@ -432,6 +432,252 @@ std::vector<torch::Tensor> flash_attn_fp8_backward(torch::Tensor q, torch::Tenso
   return {dq, dk, dv};
 }
 
+// ---------------------------------------------------------------------------
+// Paged e4m3 key/value cache and the attention over it.
+
+namespace {
+
+// Stride of dimension d for the C ABI; a dimension of one entry takes `dflt`
+// (torch may report any stride there).
+int64_t stride_or(const torch::Tensor& t, int64_t d, int64_t dflt) {
+  return t.size(d) > 1 ? t.stride(d) : dflt;
+}
+
+torch::Tensor device_i32(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
+  TORCH_CHECK(t.device().is_cpu() || t.device() == like.device(), name,
+              " must be on the cache's device (or on the host)");
+  TORCH_CHECK(at::isIntegralType(t.scalar_type(), false), name, " must hold integers");
+  return t.to(like.device(), at::kInt);
+}
+
+// Fills the cache part of a call. `keep` holds converted index tensors alive.
+void fill_cache(fa8_kv_cache& c, const torch::Tensor& k, const torch::Tensor& v,
+                const torch::Tensor& k_exp, const torch::Tensor& v_exp,
+                const torch::Tensor& page_table, const torch::Tensor& seqlens,
+                const c10::optional<torch::Tensor>& status, std::vector<torch::Tensor>& keep) {
+  for (auto* t : {&k, &v})
+    TORCH_CHECK(t->device().is_cuda() && t->scalar_type() == at::ScalarType::Float8_e4m3fn &&
+                    t->dim() == 4 && t->sizes() == k.sizes() &&
+                    (t->stride(3) == 1 || t->size(3) == 1),
+                "cache k and v must be CUDA float8_e4m3fn (pages, H_kv, page_size, D) of one "
+                "shape with unit last stride");
+  for (auto* t : {&k_exp, &v_exp})
+    TORCH_CHECK(t->scalar_type() == at::kByte && t->dim() == 3 && t->size(0) == k.size(0) &&
+                    t->size(1) == k.size(1) && t->size(2) == k.size(2) &&
+                    (t->stride(2) == 1 || t->size(2) == 1),
+                "cache k_exp and v_exp must be uint8 (pages, H_kv, page_size) with unit last "
+                "stride");
+  TORCH_CHECK(v.device() == k.device() && k_exp.device() == k.device() &&
+                  v_exp.device() == k.device(),
+              "the cache's tensors must be on one device");
+  TORCH_CHECK(page_table.dim() == 2 && seqlens.dim() == 1 &&
+                  page_table.size(0) == seqlens.size(0),
+              "page_table must be (batch, max_pages) and seqlens (batch)");
+  auto table = device_i32(page_table, k, "page_table");
+  if (table.size(1) > 1 && table.stride(1) != 1) table = table.contiguous();
+  auto lens = device_i32(seqlens, k, "seqlens").contiguous();
+  const int64_t P = k.size(0), Hkv = k.size(1), ps = k.size(2), D = k.size(3);
+  fa8_kv_cache_init(&c, P, Hkv, ps, D, table.size(0), table.size(1));
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.k_exp = k_exp.data_ptr<uint8_t>();
+  c.v_exp = v_exp.data_ptr<uint8_t>();
+  c.k_stride_p = stride_or(k, 0, c.k_stride_p);
+  c.k_stride_h = stride_or(k, 1, c.k_stride_h);
+  c.k_stride_s = stride_or(k, 2, c.k_stride_s);
+  c.v_stride_p = stride_or(v, 0, c.v_stride_p);
+  c.v_stride_h = stride_or(v, 1, c.v_stride_h);
+  c.v_stride_s = stride_or(v, 2, c.v_stride_s);
+  c.k_exp_stride_p = stride_or(k_exp, 0, c.k_exp_stride_p);
+  c.k_exp_stride_h = stride_or(k_exp, 1, c.k_exp_stride_h);
+  c.v_exp_stride_p = stride_or(v_exp, 0, c.v_exp_stride_p);
+  c.v_exp_stride_h = stride_or(v_exp, 1, c.v_exp_stride_h);
+  c.page_table = table.data_ptr<int>();
+  c.table_stride = stride_or(table, 0, table.size(1));
+  c.seqlens = lens.data_ptr<int>();
+  if (status.has_value()) {
+    TORCH_CHECK(status->device() == k.device() && status->scalar_type() == at::kInt &&
+                    status->numel() >= 1 && status->is_contiguous(),
+                "status must be a contiguous int32 CUDA tensor on the cache's device");
+    c.status = status->data_ptr<int32_t>();
+  }
+  keep.push_back(table);
+  keep.push_back(lens);
+}
+
+// 16-byte accesses: aligned base, strides of whole 8-element pieces, unit d.
+bool vec8_ok(const torch::Tensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  const int64_t last = t.dim() - 1;
+  if (t.size(last) > 1 && t.stride(last) != 1) return false;
+  for (int64_t d = 0; d < last; ++d)
+    if (t.size(d) > 1 && (t.stride(d) % 8 != 0 || t.stride(d) < 0)) return false;
+  return true;
+}
+
+int dtype_code(at::ScalarType t, const char* name) {
+  TORCH_CHECK(t == at::ScalarType::Half || t == at::ScalarType::BFloat16, name,
+              " must be fp16 or bf16, got ", t);
+  return t == at::ScalarType::Half ? FA8_DT_F16 : FA8_DT_BF16;
+}
+
+// Shapes and strides of the rows of a cache copy: packed (tokens, H_kv, D)
+// with cu_seqlens, else (batch, H_kv, tokens, D).
+void fill_rows(fa8_kv_copy_params& p, const torch::Tensor& k, const torch::Tensor& v,
+               const c10::optional<torch::Tensor>& cu_seqlens, std::vector<torch::Tensor>& keep,
+               const torch::Tensor& like) {
+  const int64_t B = p.cache.batch, Hkv = p.cache.heads_kv, D = p.cache.head_dim;
+  for (auto* t : {&k, &v}) {
+    TORCH_CHECK(t->device() == like.device(), "k and v must be on the cache's device");
+    TORCH_CHECK(t->scalar_type() == k.scalar_type() && t->sizes() == k.sizes(),
+                "k and v must have one shape and dtype");
+  }
+  p.dtype = dtype_code(k.scalar_type(), "k and v");
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  if (cu_seqlens.has_value()) {
+    TORCH_CHECK(k.dim() == 3 && k.size(1) == Hkv && k.size(2) == D,
+                "packed k and v must be (tokens, H_kv, D)");
+    TORCH_CHECK(cu_seqlens->dim() == 1 && cu_seqlens->numel() == B + 1,
+                "cu_seqlens must be 1-D with batch + 1 entries");
+    auto cu = device_i32(*cu_seqlens, like, "cu_seqlens").contiguous();
+    p.cu_seqlens = cu.data_ptr<int>();
+    keep.push_back(cu);
+    p.tokens = k.size(0);
+    p.k_stride_s = stride_or(k, 0, Hkv * D);
+    p.k_stride_h = stride_or(k, 1, D);
+    p.v_stride_s = stride_or(v, 0, Hkv * D);
+    p.v_stride_h = stride_or(v, 1, D);
+  } else {
+    TORCH_CHECK(k.dim() == 4 && k.size(0) == B && k.size(1) == Hkv && k.size(3) == D,
+                "k and v must be (batch, H_kv, tokens, D) without cu_seqlens");
+    p.tokens = k.size(2);
+    p.k_stride_b = stride_or(k, 0, Hkv * p.tokens * D);
+    p.k_stride_h = stride_or(k, 1, p.tokens * D);
+    p.k_stride_s = stride_or(k, 2, D);
+    p.v_stride_b = stride_or(v, 0, Hkv * p.tokens * D);
+    p.v_stride_h = stride_or(v, 1, p.tokens * D);
+    p.v_stride_s = stride_or(v, 2, D);
+  }
+}
+
+}  // namespace
+
+void kv_cache_write(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_exp,
+                    torch::Tensor v_exp, torch::Tensor k, torch::Tensor v,
+                    torch::Tensor page_table, torch::Tensor seqlens,
+                    c10::optional<torch::Tensor> cu_seqlens,
+                    c10::optional<torch::Tensor> status) {
+  TORCH_CHECK(k_cache.device().is_cuda(), "the cache must be on a CUDA device");
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  std::vector<torch::Tensor> keep;
+  fa8_kv_copy_params p = fa8_kv_copy_params();
+  fill_cache(p.cache, k_cache, v_cache, k_exp, v_exp, page_table, seqlens, status, keep);
+  if (!vec8_ok(k)) k = k.clone(at::MemoryFormat::Contiguous);
+  if (!vec8_ok(v)) v = v.clone(at::MemoryFormat::Contiguous);
+  fill_rows(p, k, v, cu_seqlens, keep, k_cache);
+  check_status(fa8_kv_write(&p, at::cuda::getCurrentCUDAStream(k_cache.get_device()).stream()),
+               "fa8_kv_write");
+}
+
+std::vector<torch::Tensor> kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache,
+                                         torch::Tensor k_exp, torch::Tensor v_exp,
+                                         torch::Tensor page_table, torch::Tensor seqlens,
+                                         c10::optional<torch::Tensor> cu_seqlens, int64_t tokens,
+                                         std::string dtype, c10::optional<torch::Tensor> out_k,
+                                         c10::optional<torch::Tensor> out_v,
+                                         c10::optional<torch::Tensor> status) {
+  TORCH_CHECK(k_cache.device().is_cuda(), "the cache must be on a CUDA device");
+  TORCH_CHECK(dtype == "fp16" || dtype == "bf16", "dtype must be 'fp16' or 'bf16'");
+  TORCH_CHECK(tokens >= 0, "tokens must be >= 0");
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  std::vector<torch::Tensor> keep;
+  fa8_kv_copy_params p = fa8_kv_copy_params();
+  fill_cache(p.cache, k_cache, v_cache, k_exp, v_exp, page_table, seqlens, status, keep);
+  const auto st = dtype == "fp16" ? at::ScalarType::Half : at::ScalarType::BFloat16;
+  std::vector<int64_t> shape;
+  if (cu_seqlens.has_value())
+    shape = {tokens, p.cache.heads_kv, p.cache.head_dim};
+  else
+    shape = {p.cache.batch, p.cache.heads_kv, tokens, p.cache.head_dim};
+  TORCH_CHECK(out_k.has_value() == out_v.has_value(), "out takes both k and v");
+  torch::Tensor k, v;
+  if (out_k.has_value()) {
+    k = *out_k;
+    v = *out_v;
+    for (auto* t : {&k, &v})
+      TORCH_CHECK(t->scalar_type() == st && t->sizes() == torch::IntArrayRef(shape) &&
+                      t->is_non_overlapping_and_dense() && vec8_ok(*t),
+                  "out must be dense ", dtype, " tensors of the result's shape, unit last stride, "
+                  "16-byte aligned");
+  } else {
+    k = torch::empty(shape, k_cache.options().dtype(st));
+    v = torch::empty(shape, k_cache.options().dtype(st));
+  }
+  fill_rows(p, k, v, cu_seqlens, keep, k_cache);
+  check_status(fa8_kv_read(&p, at::cuda::getCurrentCUDAStream(k_cache.get_device()).stream()),
+               "fa8_kv_read");
+  return {k, v};
+}
+
+std::vector<torch::Tensor> flash_attn_fp8_decode(
+    torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_exp,
+    torch::Tensor v_exp, torch::Tensor page_table, torch::Tensor seqlens, int64_t prefix_len,
+    c10::optional<double> softmax_scale, bool return_lse, c10::optional<torch::Tensor> out_opt,
+    c10::optional<torch::Tensor> status) {
+  TORCH_CHECK(q.device().is_cuda() && q.dim() == 4, "q must be a 4-D CUDA tensor");
+  const int dt = dtype_code(q.scalar_type(), "q");
+  TORCH_CHECK(k_cache.device() == q.device(), "q and the cache must be on the same device");
+  c10::cuda::CUDAGuard guard(q.device());
+  std::vector<torch::Tensor> keep;
+  const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3);
+  fa8_decode_params p;
+  fa8_kv_cache c;
+  fill_cache(c, k_cache, v_cache, k_exp, v_exp, page_table, seqlens, status, keep);
+  TORCH_CHECK(c.batch == B && c.head_dim == D,
+              "q must be (batch, H, S_q, D) with the cache's batch and head dimension");
+  fa8_decode_params_init(&p, c.num_pages, c.heads_kv, c.page_size, D, B, c.max_pages, H, Sq);
+  p.cache = c;
+  p.dtype = dt;
+  if (!vec8_ok(q)) q = q.clone(at::MemoryFormat::Contiguous);
+  torch::Tensor out;
+  if (out_opt.has_value()) {
+    out = *out_opt;
+    TORCH_CHECK(out.device() == q.device() && out.scalar_type() == q.scalar_type() &&
+                    out.sizes() == q.sizes() && out.is_non_overlapping_and_dense() && vec8_ok(out),
+                "out must be a dense tensor of q's shape and dtype, unit last stride, 16-byte "
+                "aligned");
+  } else {
+    out = torch::empty({B, H, Sq, D}, q.options());
+  }
+  torch::Tensor lse;
+  if (return_lse) {
+    lse = torch::empty({B, H, Sq}, q.options().dtype(at::ScalarType::Float));
+    p.lse = lse.data_ptr<float>();
+  }
+  p.q = q.data_ptr();
+  p.o = out.data_ptr();
+  p.q_stride_b = stride_or(q, 0, p.q_stride_b);
+  p.q_stride_h = stride_or(q, 1, p.q_stride_h);
+  p.q_stride_s = stride_or(q, 2, p.q_stride_s);
+  p.o_stride_b = stride_or(out, 0, p.o_stride_b);
+  p.o_stride_h = stride_or(out, 1, p.o_stride_h);
+  p.o_stride_s = stride_or(out, 2, p.o_stride_s);
+  p.prefix_len = prefix_len;
+  if (softmax_scale.has_value()) p.softmax_scale = static_cast<float>(*softmax_scale);
+  // Scratch of the current stream, taken anew for each call: calls on other
+  // streams, and captured graphs, have their own.
+  torch::Tensor ws;
+  const int64_t ws_bytes = fa8_decode_workspace_size(&p);
+  TORCH_CHECK(ws_bytes >= 0, "fa8_decode_workspace_size: ", fa8_last_error_message());
+  if (ws_bytes > 0) ws = torch::empty({ws_bytes}, q.options().dtype(at::kByte));
+  check_status(fa8_decode(&p, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
+                          at::cuda::getCurrentCUDAStream(q.get_device()).stream()),
+               "fa8_decode");
+  if (return_lse) return {out, lse};
+  return {out};
+}
+
 int64_t launch_count() { return (int64_t)fa8_launch_count(); }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -459,5 +705,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("v"), py::arg("out"), py::arg("grad_out"), py::arg("lse"),
         py::arg("causal") = true, py::arg("softmax_scale") = py::none(),
         py::arg("v_layout") = "bhds", "gradients [dq, dk, dv] (fp32) of the FP8 attention");
+  m.def("kv_cache_write", &kv_cache_write, py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("k_exp"), py::arg("v_exp"), py::arg("k"), py::arg("v"), py::arg("page_table"),
+        py::arg("seqlens"), py::arg("cu_seqlens") = py::none(), py::arg("status") = py::none(),
+        "quantise new tokens into a paged e4m3 cache");
+  m.def("kv_cache_read", &kv_cache_read, py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("k_exp"), py::arg("v_exp"), py::arg("page_table"), py::arg("seqlens"),
+        py::arg("cu_seqlens"), py::arg("tokens"), py::arg("dtype") = "fp16",
+        py::arg("out_k") = py::none(), py::arg("out_v") = py::none(),
+        py::arg("status") = py::none(), "read cached tokens back as fp16 / bf16: [k, v]");
+  m.def("flash_attn_fp8_decode", &flash_attn_fp8_decode, py::arg("q"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("k_exp"), py::arg("v_exp"), py::arg("page_table"),
+        py::arg("seqlens"), py::arg("prefix_len") = 0, py::arg("softmax_scale") = py::none(),
+        py::arg("return_lse") = false, py::arg("out") = py::none(),
+        py::arg("status") = py::none(),
+        "attention of each sequence's last tokens over its cache; returns [out] or [out, lse]");
   m.def("launch_count", &launch_count, "kernel launches issued by the C ABI so far");
 }

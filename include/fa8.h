@@ -17,6 +17,9 @@
  *                     gradient of the same attention for training callers.
  *   fa8_lse_merge  <- no counterpart in the reference (which emits no LSE);
  *                     merges partial outputs of the context-parallel ring.
+ *   fa8_kv_write, fa8_kv_read, fa8_decode <- no counterpart in the reference
+ *                     (no cache, no form for single tokens): a paged e4m3
+ *                     key/value cache and the attention that reads it.
  *   fa8_quantize_e4m3 <- the torch casts that prepare the kernel inputs in
  *                     test.py:35-37 and the V transpose at test.py:51-52.
  */
@@ -54,8 +57,19 @@ enum { FA8_OUT_F16 = 0, FA8_OUT_E4M3 = 1, FA8_OUT_F32 = 2 };
  * faulting or hanging: a bounded wait gave up (TIMEOUT), a varlen sequence
  * whose K/V start is not a multiple of 16 (VARLEN_ALIGN), or a varlen
  * sequence whose offsets leave the packed tensors or that is longer than
- * max_seqlen_q (VARLEN_RANGE). A refused sequence is left unwritten. */
-enum { FA8_DEVERR_TIMEOUT = 1, FA8_DEVERR_VARLEN_ALIGN = 2, FA8_DEVERR_VARLEN_RANGE = 4 };
+ * max_seqlen_q (VARLEN_RANGE; for the cache entry points a sequence whose
+ * length does not fit its page table or its new tokens). A refused sequence
+ * is left unwritten. PAGE_RANGE: a page id outside the cache was needed; its
+ * tokens are not written, read back as NaN and make their queries NaN. */
+enum {
+  FA8_DEVERR_TIMEOUT = 1,
+  FA8_DEVERR_VARLEN_ALIGN = 2,
+  FA8_DEVERR_VARLEN_RANGE = 4,
+  FA8_DEVERR_PAGE_RANGE = 8
+};
+
+/* 16-bit element types of fa8_quantize_e4m3, the cache and the decode. */
+enum { FA8_DT_F16 = 0, FA8_DT_BF16 = 1 };
 
 /*
  * All strides are in ELEMENTS. Tensors are indexed [b][h][s][d] for Q, K and
@@ -273,6 +287,118 @@ void fa8_bwd_params_init(fa8_bwd_params* p, int64_t batch, int64_t heads, int64_
                          int64_t seqlen_q, int64_t seqlen_kv, int64_t head_dim);
 int64_t fa8_bwd_workspace_size(const fa8_bwd_params* p);
 int fa8_bwd(const fa8_bwd_params* p, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * A paged e4m3 key/value cache and the sequences held in it (no counterpart
+ * in the reference). Codes are indexed [page][kv head][slot][d] with strides
+ * in elements, d of unit stride, the others multiples of 16 (any order: a
+ * cache stored [page][slot][head][d] is one with other strides). Every (page,
+ * head, slot) of K and of V has an exponent byte, indexed [page][head][slot]
+ * with unit slot stride: value = code * 2^(byte - 127); 255 marks a row that
+ * held an infinity or a NaN and reads as NaN. Token t of sequence b lies in
+ * slot t % page_size of page page_table[b * table_stride + t / page_size];
+ * the sequence holds seqlens[b] tokens. Tables and lengths are read on the
+ * device only. page_size: 16, 32, 64 or a multiple of 128.
+ */
+typedef struct fa8_kv_cache {
+  void* k;
+  void* v;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  int64_t num_pages;
+  int64_t heads_kv;
+  int64_t page_size;
+  int64_t head_dim;         /* 64 or 128                                     */
+  int64_t k_stride_p, k_stride_h, k_stride_s;
+  int64_t v_stride_p, v_stride_h, v_stride_s;
+  int64_t k_exp_stride_p, k_exp_stride_h;
+  int64_t v_exp_stride_p, v_exp_stride_h;
+  int64_t batch;
+  const int32_t* page_table; /* device, [batch][max_pages]                   */
+  int64_t table_stride;
+  int64_t max_pages;         /* table columns: a sequence holds at most
+                                max_pages * page_size tokens                 */
+  const int32_t* seqlens;    /* device, [batch]                              */
+  int32_t* status;           /* optional device word, FA8_DEVERR_* bits      */
+} fa8_kv_cache;
+
+/* Fill *c for contiguous [page][head][slot][d] codes and [page][head][slot]
+ * exponents and a contiguous [batch][max_pages] table. */
+void fa8_kv_cache_init(fa8_kv_cache* c, int64_t num_pages, int64_t heads_kv, int64_t page_size,
+                       int64_t head_dim, int64_t batch, int64_t max_pages);
+
+/*
+ * The last n_b tokens of every sequence, positions seqlens[b] - n_b ..
+ * seqlens[b] - 1, as fp16 or bf16 rows. Without cu_seqlens k and v are
+ * [batch][kv head][tokens][d] and n_b = tokens. With cu_seqlens (device int32
+ * prefix sums, batch + 1 entries) they are packed, [tokens][kv head][d] with
+ * tokens rows in all (strides _s and _h; _b unused) and n_b = cu_seqlens[b + 1]
+ * - cu_seqlens[b]; rows outside cu_seqlens[0] .. cu_seqlens[batch] are not
+ * touched. Strides in elements, multiples of 8, d of unit stride, bases
+ * 16-byte aligned.
+ */
+typedef struct fa8_kv_copy_params {
+  fa8_kv_cache cache;
+  void* k;                  /* read by fa8_kv_write, written by fa8_kv_read  */
+  void* v;
+  const int32_t* cu_seqlens; /* or NULL                                      */
+  int64_t tokens;
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  int64_t v_stride_b, v_stride_h, v_stride_s;
+  int32_t dtype;            /* FA8_DT_F16 or FA8_DT_BF16                     */
+  int32_t reserved0;
+} fa8_kv_copy_params;
+
+/* Quantise the tokens into the cache. Each row of d elements gets the least
+ * exponent e >= -63 with max|x| <= 448 * 2^e (0 for a row of zeros) and the
+ * codes rn_e4m3(x * 2^-e); a row with an infinity or a NaN gets byte 255 and
+ * zero codes. No two tokens of a call may share a slot (sequences may share
+ * pages that the call only leaves alone). */
+int fa8_kv_write(const fa8_kv_copy_params* p, void* stream);
+/* Read them back: code * 2^(byte - 127), rounded once to dtype, saturating. */
+int fa8_kv_read(const fa8_kv_copy_params* p, void* stream);
+
+/*
+ * Attention of the last seqlen_q tokens of every sequence over its cached
+ * keys: query i of sequence b has position n = seqlens[b] - seqlen_q + i and
+ * sees keys 0 .. n (its own K and V are in the cache already). q and o are
+ * [batch][heads][seqlen_q][d] of type dtype (strides in elements, unit d;
+ * those of q and o multiples of 8, bases 16-byte aligned); lse (optional) is
+ * fp32 [batch][heads][seqlen_q], natural log, contiguous. Queries that see no
+ * key give o = 0 and lse = -inf.
+ *
+ * prefix_len > 0: the first prefix_len tokens of all sequences are the same
+ * and are read once for the whole batch, from the pages of row 0 of the
+ * table (the caller vouches for it; no other row's pages are read for them).
+ * The result is that of prefix_len = 0.
+ *
+ * The caller provides fa8_decode_workspace_size() bytes of device workspace,
+ * 256-byte aligned; nothing in it is kept or expected between calls, and
+ * calls that may run at the same time need one each.
+ */
+typedef struct fa8_decode_params {
+  fa8_kv_cache cache;
+  const void* q;
+  void* o;
+  float* lse;               /* may be NULL */
+  int64_t heads;            /* multiple of cache.heads_kv */
+  int64_t seqlen_q;
+  int64_t q_stride_b, q_stride_h, q_stride_s;
+  int64_t o_stride_b, o_stride_h, o_stride_s;
+  int64_t prefix_len;
+  float softmax_scale;      /* natural-log scale, usually 1/sqrt(head_dim)   */
+  int32_t dtype;            /* of q and o: FA8_DT_F16 or FA8_DT_BF16         */
+  int64_t wait_timeout_cycles; /* bound of every wait; <= 0: ~2 s            */
+} fa8_decode_params;
+
+/* Contiguous q and o, scale 1/sqrt(head_dim), fp16, no prefix. The cache part
+ * is filled by fa8_kv_cache_init. */
+void fa8_decode_params_init(fa8_decode_params* p, int64_t num_pages, int64_t heads_kv,
+                            int64_t page_size, int64_t head_dim, int64_t batch,
+                            int64_t max_pages, int64_t heads, int64_t seqlen_q);
+/* Host-only; depends on the sizes alone, not on lengths or pointers. */
+int64_t fa8_decode_workspace_size(const fa8_decode_params* p);
+int fa8_decode(const fa8_decode_params* p, void* workspace, int64_t workspace_bytes, void* stream);
 
 const char* fa8_status_string(int status);
 const char* fa8_last_error_message(void);
