@@ -146,7 +146,7 @@ class KVCacheFP8(NamedTuple):
     ``k``, ``v``: float8_e4m3fn (pages, H_kv, page_size, D), unit last stride, the
     other strides multiples of 16 (a (pages, page_size, H_kv, D) tensor is passed as
     its ``transpose(1, 2)``); ``k_exp``, ``v_exp``: uint8 (pages, H_kv, page_size),
-    unit last stride. The row of a token and head has the values
+    unit last stride, the others multiples of 16. The row of a token and head has the values
     ``code * 2**(exp - 127)``; 255 marks a row that held an infinity or a NaN and
     reads as NaN. page_size is 16, 32, 64 or a multiple of 128, D 64 or 128.
     """

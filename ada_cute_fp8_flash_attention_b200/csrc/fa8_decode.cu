@@ -30,15 +30,14 @@
 //
 // Softmax in base 2 with one running maximum per row, m = max(s + e), e the
 // exponent of v_j: then p = 2^(s - m) enters the sum, and what goes to the
-// product is 2^5 * 2^(e) * p <= 2^5 whatever the exponents are (times 2^3,
-// the rise of the maximum below which nothing is rescaled). The sum is kept
+// product is 2^3 * 2^e * p <= 2^3 whatever the exponents are (times 2^5, the
+// rise of the maximum below which nothing is rescaled). The sum is kept
 // per thread, over its own keys, and joined at the end of a row's keys.
 //
 // Work. Key tiles of 128 of all (sequence, K/V head, tile of query rows) are
-// numbered through; block c of G = min(blocks, U) takes those from U c / G to
-// U (c + 1) / G,
-// found from the lengths on the device by a scan: any mixture of lengths
-// shares the GPU evenly and nothing is read on the host. A block that holds
+// numbered through and every block takes an equal run of them, which it finds
+// from the lengths on the device by a scan: any mixture of lengths shares the
+// GPU evenly and nothing is read on the host. A block that holds
 // all of an item's keys writes the result; else it writes its unnormalised
 // sums, and a second kernel, launched early and waiting on the device for the
 // first, joins them (always the same shares: results repeat bit by bit).
@@ -55,6 +54,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "fa8_kv.cuh"
 #include "sm100_ptx.cuh"
@@ -63,8 +63,8 @@ namespace fa8 {
 namespace dec {
 
 constexpr int kTileKeys = 128;
-constexpr float kRise = 3.f;           // log2 of the rise of a maximum that is let be
-constexpr float kPScale = 32.f;        // 2^5 p 2^e <= 2^(5 + kRise) < 448
+constexpr float kRise = 5.f;           // log2 of the rise of a maximum that is let be
+constexpr float kPScale = 8.f;         // 8 p 2^e <= 2^(3 + kRise) < 448
 constexpr float kTerm = 16.f;          // weight of a term over the next
 constexpr long long kTimeout = 4000000000LL;
 constexpr int kWaitHintNs = 20000;
@@ -79,9 +79,11 @@ template <int D_, int NT_, int RW_, int NWG_>
 struct Cfg {
   static constexpr int D = D_, NT = NT_, RW = RW_, NWG = NWG_;
   static constexpr int kRows = RW * NWG;
-  static constexpr int kThreads = NWG * 128 + 64;
-  static constexpr int kMmaWarp = NWG * 4, kLoadWarp = NWG * 4 + 1;
+  static constexpr int kThreads = NWG * 128 + 128;
+  static constexpr int kMmaWarp = NWG * 4, kLoadWarp = NWG * 4 + 1, kQWarp = NWG * 4 + 2;
+  static constexpr int kQWarps = 2;
   static constexpr int kN = (NT * RW + 15) / 16 * 16;  // columns of the products
+  static constexpr int kStep = RW < 16 ? 8 : 16;       // rows read from TMEM at a time
   static constexpr int kPitch = kN <= 64 ? 64 : 128;   // bytes of a key's row of P
   static constexpr int kSlotBytes = kTileKeys * D;     // a K or a V tile
   static constexpr int kQBytes = kN * D;               // per warpgroup
@@ -89,13 +91,27 @@ struct Cfg {
   static constexpr uint32_t kTmemUsed = 2u * kN * NWG;
   static constexpr uint32_t kTmemCols =
       kTmemUsed <= 32 ? 32 : kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
-  static constexpr int kCtas = NWG > 1 ? 1 : (D == 64 && RW <= 16 ? 3 : 2);  // per SM
-  static constexpr int kFixed = NWG * (kQBytes + kPBytes);
+  static constexpr int kCtas = NWG > 1 ? 1 : (D == 64 && RW == 8 ? 3 : 2);  // per SM
   // 227 KB a block, 228 KB an SM of which each block takes 1 KB and its
   // static variables; 1 KB to align.
-  static constexpr int kBudget = (kCtas == 1 ? 227 : (228 - kCtas) / kCtas) * 1024 - 4096 - 1024;
-  static constexpr int kSlots = (kBudget - kFixed) / kSlotBytes < 12 ? (kBudget - kFixed) / kSlotBytes : 12;
-  static constexpr int kSmem = kSlots * kSlotBytes + kFixed + 1024;
+  static constexpr int kStatic = 2688 + 80 * kRows;
+  static constexpr int kBudget = (kCtas == 1 ? 227 : (228 - kCtas) / kCtas) * 1024 - kStatic - 1024;
+  // P in two buffers where four tiles of the ring still fit beside them: the
+  // next one is then written while the product of this one runs.
+  static constexpr int slots_with(int bufs) {
+    const int n = (kBudget - NWG * (2 * kQBytes + bufs * kPBytes)) / kSlotBytes;
+    return n < 12 ? n : 12;
+  }
+  static constexpr int kPBufs = slots_with(2) >= 4 ? 2 : 1;
+  static constexpr int kSlots = slots_with(kPBufs);
+  static constexpr int kSmem = kSlots * kSlotBytes + NWG * (2 * kQBytes + kPBufs * kPBytes) + 1024;
+  // Registers: what the launch bounds give a thread, moved from the helpers
+  // (loads, products, Q) to the softmax warpgroups.
+  static constexpr int kRegsLaunch = 65536 / (kCtas * kThreads) / 8 * 8;
+  static constexpr int kRegsHelp = kCtas == 3 ? 56 : (NWG > 1 ? 88 : 72);
+  static constexpr int kRegsSoft = ((NWG + 1) * kRegsLaunch - kRegsHelp) / NWG / 8 * 8;
+  static_assert(NWG * kRegsSoft + kRegsHelp <= (NWG + 1) * kRegsLaunch && kRegsSoft <= 255,
+                "setmaxnreg must not ask for more than the block was launched with");
   static_assert(kTmemUsed <= 512 && kTmemCols * kCtas <= 512, "TMEM of the resident blocks");
   static_assert(kSlots >= 4, "a K and a V tile in use and two on their way");
   static_assert(RW == 8 || RW == 16 || RW == 32, "rows of a warpgroup");
@@ -115,7 +131,7 @@ struct Args {
   int prefix_len;
   int row_tiles;     // tiles of query rows per (sequence, K/V head)
   int box;           // keys of a TMA box: min(page_size, 128)
-  int page_shift;    // log2(page_size), or -1
+  uint32_t page_mul, page_shift;  // key / page_size = (mulhi(key, mul) + key) >> shift
   int own_rows;      // results go to o (1), or to full_* and item (0)
   int early;         // this launch may overlap the one before it
   float scale_log2;
@@ -224,6 +240,8 @@ __device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
   return d;
 }
 
+__device__ __forceinline__ float sum_of(const float4& v) { return (v.x + v.y) + (v.z + v.w); }
+
 // -------------------------------------------------------------------- waiting
 // Every wait is bounded. One that gave up sets the block's abort flag, which
 // ends all others; each role then leaves its loop.
@@ -234,6 +252,7 @@ struct Waiter {
   __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
+#pragma unroll 1
     while (!ptx::mbar_try_wait_sleep(bar, parity, kWaitHintNs)) {
       if (*abort) return false;
       if (clock64() - t0 > limit) {
@@ -268,27 +287,16 @@ __device__ __forceinline__ int tiles_of(const Args& a, int len) {
 // A run of key tiles t0..t1-1 of one item (sequence b, K/V head, row tile).
 struct Seg {
   int b, hk, rt, t0, t1, nt, len;
-  long long unit;  // number of tile t0 among all
+  int unit;  // number of tile t0 among all
 };
 
 // Walks a block's share of the tiles; every role of the block walks the same.
 struct Walk {
   int b, hk, rt, t, nt, len;
-  long long unit, left;
+  int unit, left;
   __device__ __forceinline__ void enter(const Args& a) {
     len = seq_len(a, b);
     nt = tiles_of(a, len);
-  }
-  __device__ __forceinline__ void begin(const Args& a, int b0, long long off, long long unit0,
-                                        long long units) {
-    b = b0;
-    unit = unit0;
-    left = units;
-    enter(a);
-    const long long j = off / nt;
-    t = (int)(off - j * nt);
-    hk = (int)(j / a.row_tiles);
-    rt = (int)(j - (long long)hk * a.row_tiles);
   }
   __device__ __forceinline__ bool next(const Args& a, Seg& s) {
     if (left == 0) return false;
@@ -302,9 +310,9 @@ struct Walk {
     s.t0 = t;
     s.nt = nt;
     s.len = len;
-    s.t1 = (int)min((long long)nt, t + left);
+    const int n = min(nt - t, left);
+    s.t1 = t + n;
     s.unit = unit;
-    const int n = s.t1 - s.t0;
     left -= n;
     unit += n;
     t = s.t1;
@@ -323,106 +331,180 @@ struct Walk {
   }
 };
 
+// Shares of `total` tiles over `n` blocks: the first total % n have one more.
+struct Shares {
+  int size, more;
+  __device__ __forceinline__ Shares(int total, int n) : size(total / n), more(total - size * n) {}
+  __device__ __forceinline__ int begin(int c) const { return c * size + min(c, more); }
+  __device__ __forceinline__ int block_of(int unit) const {
+    const int wide = more * (size + 1);
+    return unit < wide ? unit / (size + 1) : more + (unit - wide) / size;
+  }
+};
+
 __device__ __forceinline__ int page_of(const Args& a, int key) {
-  return a.page_shift >= 0 ? key >> a.page_shift : key / a.c.page_size;
+  return (int)((__umulhi((uint32_t)key, a.page_mul) + (uint32_t)key) >> a.page_shift);
 }
+
+constexpr int kExpTiles = 8;  // ring of exponent bytes: tiles in flight and two more
 
 template <class C>
 struct __align__(16) Shared {
+  uint8_t exps[kExpTiles][2][kTileKeys];  // of K and V
   uint64_t kv_full[C::kSlots];
   uint64_t kv_empty[C::kSlots];
-  uint64_t q_full[C::NWG];
-  uint64_t s_full[C::NWG];   // S^T in TMEM
-  uint64_t s_free[C::NWG];   // read by the four warps
-  uint64_t p_full[C::NWG];   // P^T in shared memory (and O^T rescaled)
-  uint64_t o_done[C::NWG];   // O^T += V^T P^T complete
-  uint64_t meet[C::NWG];     // the four warps of a warpgroup
+  uint64_t e_full[kExpTiles];
+  uint64_t q_full[2];        // Q and row data of an item, two items in turn
+  uint64_t q_free[2];
+  uint64_t s_full;           // S^T of all warpgroups in TMEM
+  uint64_t s_free;           // read by their warps, and the tile's exponents
+  // P^T in shared memory (and O^T rescaled), tiles in turn: the softmax may be
+  // done with tile n + 1 before the products have looked for tile n, but not
+  // with tile n + 2, whose scores are issued behind the values of tile n.
+  uint64_t p_full[C::NWG][2];
+  uint64_t o_done[C::NWG][2];  // O^T += V^T P^T complete, tiles in turn
   uint64_t drain;
   uint32_t tmem;
   int abort;
-  int b0;
-  long long off0;
-  long long warp_units[16];
+  struct __align__(16) Rows {  // of an item; read four at a time
+    float mul[C::kRows];     // scale * log2(e) * the power of two of the row of Q
+    int row_id[C::kRows];    // (b * heads + h) * seqlen_q + i; -1: no such row
+    int lim[C::kRows];       // keys that the row sees
+    long long off[C::kRows]; // where a whole row's result goes, in elements
+    int all_see[C::kQWarps]; // keys that all rows of a Q warp see
+  } rows[2];
   struct Group {
-    float mul[C::RW];        // scale * log2(e) * the power of two of the row of Q
-    float inv[C::RW];
-    float sum[4][C::RW];
-    float top[2][4][C::RW];  // warps' maxima of a tile, two tiles in turn
-    long long o_off[C::RW];  // element offset of the row in o; -1: none
-    int row_id[C::RW];       // (b * heads + h) * seqlen_q + i
-    int lim[C::RW];          // keys that the row sees
+    float neg_m[C::RW];      // minus the running maxima
+    float step[C::RW];       // and what the last rise added to that
+    float4 sum[C::RW];       // the four warps' sums of a row
+    float4 top[C::RW];       // and maxima of a tile
   } g[C::NWG];
+  static_assert(sizeof(Rows) % 16 == 0 && sizeof(Group) % 16 == 0, "read four at a time");
+  static_assert(C::kSlots / 2 + 2 <= kExpTiles, "a tile's exponents are read before their place is used again");
 };
+
+// Row j of item rows (K/V head hk; sequence b unless the items are the
+// prefix's): its sequence, head and query.
+struct Row {
+  int b, h, i;
+  __device__ __forceinline__ Row(const Args& a, int seq, int hk, int j) {
+    const int n = a.seqlen_q * a.group;
+    b = seq;
+    if (a.prefix_mode) {
+      b = j / n;
+      j -= b * n;
+    }
+    i = j / a.group;
+    h = hk * a.group + j - i * a.group;
+  }
+};
+
+// Sums over the warp of N values per lane: lane l has that of value
+// l / (32 / N). Every step halves the values a lane keeps.
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int half = N / 2, o = 16; half; half >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+#pragma unroll
+  for (int o = 16 / N; o; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
 
 template <class C, bool kBf16>
 __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                   const Args a) {
   constexpr int D = C::D, NT = C::NT, RW = C::RW, NS = C::kSlots;
+  static_assert(sizeof(Shared<C>) <= C::kStatic, "shared memory budget");
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared<C> sh;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int G = gridDim.x, cta = blockIdx.x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ------------------------------------------------- this block's share
-  const int nseq = a.prefix_mode ? 1 : a.c.batch;
-  const int chunk = (nseq + C::kThreads - 1) / C::kThreads;
-  const int s0 = min(nseq, (int)threadIdx.x * chunk), s1 = min(nseq, s0 + chunk);
-  const long long per = (long long)a.c.heads_kv * a.row_tiles;
-  long long mine = 0;
-  for (int b = s0; b < s1; ++b) {
-    const int len = seq_len(a, b);
-    if (len < 0 && cta == 0 && a.c.status) atomicOr(a.c.status, FA8_DEVERR_VARLEN_RANGE);
-    mine += per * tiles_of(a, len);
-  }
-  long long upto = mine;  // inclusive scan
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) sh.warp_units[warp] = upto;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < NS; ++s) {
-      ptx::mbar_init(&sh.kv_full[s], 1);
-      ptx::mbar_init(&sh.kv_empty[s], 1);
+  if (warp == 0) {
+    for (int i = lane; i < NS; i += 32) {
+      ptx::mbar_init(&sh.kv_full[i], 1);
+      ptx::mbar_init(&sh.kv_empty[i], 1);
     }
-    for (int w = 0; w < C::NWG; ++w) {
-      ptx::mbar_init(&sh.q_full[w], 4);
-      ptx::mbar_init(&sh.s_full[w], 1);
-      ptx::mbar_init(&sh.s_free[w], 4);
-      ptx::mbar_init(&sh.p_full[w], 4);
-      ptx::mbar_init(&sh.o_done[w], 1);
-      ptx::mbar_init(&sh.meet[w], 4);
+    if (lane < kExpTiles) ptx::mbar_init(&sh.e_full[lane], 32);
+    if (lane < 2) {
+      ptx::mbar_init(&sh.q_full[lane], C::kQWarps);
+      ptx::mbar_init(&sh.q_free[lane], C::NWG * 4);
     }
-    ptx::mbar_init(&sh.drain, 1);
-    sh.abort = 0;
+    if (lane < C::NWG) {
+      ptx::mbar_init(&sh.p_full[lane][0], 4);
+      ptx::mbar_init(&sh.p_full[lane][1], 4);
+      ptx::mbar_init(&sh.o_done[lane][0], 1);
+      ptx::mbar_init(&sh.o_done[lane][1], 1);
+    }
+    if (lane == 0) {
+      ptx::mbar_init(&sh.s_full, 1);
+      ptx::mbar_init(&sh.s_free, C::NWG * 4);
+      ptx::mbar_init(&sh.drain, 1);
+      sh.abort = 0;
+    }
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
   }
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < C::kThreads / 32; ++w) {
-    const long long v = sh.warp_units[w];
-    if (w < warp) upto += v;
-    total += v;
+
+  // ------------------------------------------------- this block's share
+  // Every warp finds it for itself: lane i counts the tiles of a run of
+  // sequences, a scan says how many come before. (The host has checked that
+  // they number less than 2^31.)
+  const int nseq = a.prefix_mode ? 1 : a.c.batch;
+  const int chunk = (nseq + 31) / 32;
+  const int s0 = min(nseq, lane * chunk), s1 = min(nseq, s0 + chunk);
+  const int per = a.c.heads_kv * a.row_tiles;
+  int mine = 0;
+#pragma unroll 4
+  for (int b = s0; b < s1; ++b) {
+    const int len = seq_len(a, b);
+    if (len < 0 && cta == 0 && warp == 0 && a.c.status)
+      atomicOr(a.c.status, FA8_DEVERR_VARLEN_RANGE);
+    mine += per * tiles_of(a, len);
   }
-  const long long shares = min((long long)G, total);  // blocks with work: a tile at least
-  const long long u0 = cta < shares ? total * cta / shares : 0;
-  const long long u1 = cta < shares ? total * (cta + 1) / shares : 0;
-  if (u0 < u1 && u0 >= upto - mine && u0 < upto) {
-    long long at = upto - mine;
-    int b = s0;
-    while (true) {
-      const long long n = per * tiles_of(a, seq_len(a, b));
-      if (u0 < at + n) break;
-      at += n;
-      ++b;
+  if (warp == C::kMmaWarp) {
+    ptx::tmem_alloc(&sh.tmem, C::kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  int upto = mine;  // inclusive scan
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  const int total = __shfl_sync(0xffffffffu, upto, 31);
+  const int active = min(G, total);  // blocks with work: a tile at least
+  const Shares shares(total, max(active, 1));
+  const int u0 = cta < active ? shares.begin(cta) : 0;
+  const int u1 = cta < active ? shares.begin(cta + 1) : 0;
+  Walk walk;
+  walk.left = u1 - u0;
+  walk.unit = u0;
+  {
+    const uint32_t here = __ballot_sync(0xffffffffu, u0 >= upto - mine && u0 < upto);
+    const int src = __ffs(here) - 1;  // the lane in whose sequences tile u0 is
+    if (u0 < u1) {
+      int at = __shfl_sync(0xffffffffu, upto - mine, src);
+      for (walk.b = __shfl_sync(0xffffffffu, s0, src);; ++walk.b) {
+        walk.enter(a);
+        if (u0 < at + per * walk.nt) break;
+        at += per * walk.nt;
+      }
+      const int item = (u0 - at) / walk.nt;
+      walk.t = u0 - at - item * walk.nt;
+      walk.hk = item / a.row_tiles;
+      walk.rt = item - walk.hk * a.row_tiles;
     }
-    sh.b0 = b;
-    sh.off0 = u0 - at;
   }
 
   // Sequences without a key among these items have no tile and no block of
@@ -441,40 +523,43 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         }
       } else {
         for (int j = threadIdx.x; j < per; j += C::kThreads)
-          a.item[b * per + j] = make_int4(0, 0, 0, kItemEmpty);
+          a.item[(long long)b * per + j] = make_int4(0, 0, 0, kItemEmpty);
       }
     }
   }
   if (a.own_rows && threadIdx.x == 0) a.seg[cta] = make_int4(-1, 0, 0, 0);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = sh.tmem;
   if (u0 == u1) {
+    if (warp == C::kMmaWarp) ptx::tmem_dealloc(tmem, C::kTmemCols);
     if (a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  // Ring of K and V tiles | P of each warpgroup | Q of each warpgroup.
+  // Ring of K and V tiles | P of each warpgroup | Q of two items, each of all
+  // warpgroups.
   uint8_t* const p_tiles = smem + NS * C::kSlotBytes;
-  uint8_t* const q_tiles = p_tiles + C::NWG * C::kPBytes;
-  if (warp == C::kMmaWarp) {
-    ptx::tmem_alloc(&sh.tmem, C::kTmemCols);
-    ptx::tmem_relinquish();
-  }
-  ptx::tc_fence_before();
-  __syncthreads();
-  ptx::tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  uint8_t* const q_tiles = p_tiles + C::NWG * C::kPBufs * C::kPBytes;
   const Waiter wait{&sh.abort, a.c.status, a.timeout};
-  Walk walk;
-  walk.begin(a, sh.b0, sh.off0, u0, u1 - u0);
   Seg s;
 
+  if (warp >= C::kMmaWarp) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsHelp));
   if (warp == C::kLoadWarp) {
     // ------------------------------------------------------------ TMA producer
     // Lane l brings piece l (box keys of one page) of a K and of a V tile.
-    // Ring item 2n is K of the block's tile n, 2n + 1 its V.
+    // Ring item 2n is K of the block's tile n, 2n + 1 its V. Lanes 0-15 bring
+    // the tile's exponent bytes, 16 keys of K or V each.
     const int pieces = kTileKeys / a.box;
     const uint64_t policy = a.row_tiles > 1 ? ptx::policy_evict_last() : ptx::policy_evict_first();
+    const bool is_v = lane >= 8;
+    const int e_key = (lane & 7) * 16, e_piece = e_key / a.box;
+    const uint8_t* const exps = is_v ? a.c.v_exp : a.c.k_exp;
+    const long long e_sp = is_v ? a.c.ve_sp : a.c.ke_sp, e_sh = is_v ? a.c.ve_sh : a.c.ke_sh;
     if (lane == 0) {
       ptx::tma_prefetch_desc(&tm_k);
       ptx::tma_prefetch_desc(&tm_v);
@@ -490,12 +575,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       int page = entry(s.t0);
       for (int t = s.t0; t < s.t1; ++t, ++n) {
         const int next = t + 1 < s.t1 ? entry(t + 1) : 0;
-        const int key = a.key_base + t * kTileKeys + lane * a.box;
+        const int key0 = a.key_base + t * kTileKeys, key = key0 + lane * a.box;
         const bool have = lane < pieces && key < s.len;
-        // A page outside the cache: coordinates that read as zeros.
-        const int coord = page < 0 || page >= a.c.num_pages ? 0x7fffffff : page;
+        // A page outside the cache: coordinates that read as zeros, exponents
+        // that say NaN.
+        const bool outside = page < 0 || page >= a.c.num_pages;
+        if (have && outside && a.c.status) atomicOr(a.c.status, FA8_DEVERR_PAGE_RANGE);
+        const int coord = outside ? 0x7fffffff : page;
         const int slot = key - page_of(a, key) * a.c.page_size;
         const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, have)) * a.box * D;
+        const int e_coord = __shfl_sync(0xffffffffu, coord, e_piece);
+        const int e_slot = __shfl_sync(0xffffffffu, slot, e_piece) + e_key - e_piece * a.box;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
           const int i = 2 * n + v, st = i % NS;
@@ -509,324 +599,420 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             ptx::tma_load_4d(smem + st * C::kSlotBytes + lane * a.box * D, v ? &tm_v : &tm_k,
                              &sh.kv_full[st], 0, slot, s.hk, coord, policy);
           issued = i + 1;
+          if (v == 0) {
+            // K's place is free: the scores of kSlots / 2 tiles ago are done,
+            // so the tile before that has been read, exponents included.
+            uint8_t* const dst = &sh.exps[n % kExpTiles][is_v][e_key];
+            uint64_t* const bar = &sh.e_full[n % kExpTiles];
+            const bool mine = lane < 16 && key0 + e_key < s.len;
+            if (mine && e_coord == 0x7fffffff) {
+              *reinterpret_cast<uint4*>(dst) = make_uint4(~0u, ~0u, ~0u, ~0u);
+              ptx::mbar_arrive(bar);
+            } else {
+              if (mine)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)),
+                             "l"(exps + e_coord * e_sp + s.hk * e_sh + e_slot)
+                             : "memory");
+              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                               ptx::smem_u32(bar))
+                           : "memory");
+            }
+          }
         }
         if (!ok) break;
         page = next;
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok && lane == 0) {
       // Copies in flight land before the block ends.
       for (int i = max(0, issued - NS); i < issued; ++i)
         wait_quietly(&sh.kv_full[i % NS], (i / NS) & 1, a.timeout);
+    }
+  } else if (warp >= C::kQWarp) {
+    // ------------------------------------------------------------ rows and Q
+    // One item ahead of the others: row data, and Q as terms, K-major. Each of
+    // the two warps takes every other batch of rows.
+    constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row; rows at a time
+    constexpr int kHalf = C::kRows / C::kQWarps / kPer;
+    constexpr int kMost = C::NWG > 1 ? 8 : 4;           // loads in flight
+    constexpr int kBatch = kHalf < kMost ? kHalf : kMost;
+    static_assert(C::kRows % (kPer * kBatch * C::kQWarps) == 0, "whole batches");
+    const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
+    const int me = warp - C::kQWarp;
+    for (int k = 0; walk.next(a, s); ++k) {
+      const int buf = k & 1;
+      if (k >= 2 && !wait.warp(&sh.q_free[buf], ((k >> 1) - 1) & 1)) break;
+      auto& rw = sh.rows[buf];
+      const int row0 = s.rt * C::kRows, used = min(C::kRows, rows - row0);
+      // Rows up to a whole step are computed with: zeros.
+      const int filled = (used + C::kStep - 1) / C::kStep * C::kStep;
+      const int cl = lane % kLanes;
+      uint4 xs[kBatch];
+      auto ask = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int r = r0 + u * kPer + lane / kLanes;
+          xs[u] = make_uint4(0, 0, 0, 0);
+          if (r < used) {
+            const Row row(a, s.b, s.hk, row0 + r);
+            xs[u] = __ldg(reinterpret_cast<const uint4*>(
+                              a.q + 2 * (row.b * a.q_sb + row.h * a.q_sh + row.i * a.q_ss)) + cl);
+          }
+        }
+      };
+      ask(me * kPer * kBatch);  // on their way while the row data is made
+      int see = s.len;
+#pragma unroll 1
+      for (int r = me * 32 + lane; r < C::kRows; r += 64) {
+        int lim = s.len, id = -1;
+        long long off = 0;
+        if (r < used) {
+          const Row row(a, s.b, s.hk, row0 + r);
+          int len = s.len;
+          if (a.prefix_mode) {
+            len = __ldg(a.c.seqlens + row.b);
+            if (len > a.c.max_len) len = 0;  // refused: its rows are not joined
+          }
+          lim = max(0, min(s.len, len - a.seqlen_q + row.i + 1));
+          id = (row.b * a.heads + row.h) * a.seqlen_q + row.i;
+          off = a.own_rows ? row.b * a.o_sb + row.h * a.o_sh + row.i * a.o_ss : (long long)id * D;
+        }
+        rw.lim[r] = lim;
+        rw.row_id[r] = id;
+        rw.off[r] = off;
+        see = min(see, lim);
+      }
+      see = __reduce_min_sync(0xffffffffu, see);
+      if (lane == 0) rw.all_see[me] = see;
+#pragma unroll 1
+      for (int r0 = me * kPer * kBatch; r0 < filled; r0 += C::kQWarps * kPer * kBatch) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int r = r0 + u * kPer + lane / kLanes;
+          const uint4 x = xs[u];
+          uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+          m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+          for (int o = kLanes / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const bool fine = m < (kBf16 ? 0x7f80u : 0x7c00u);
+          const uint32_t bits =
+              kBf16 ? m << 16
+                    : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+          // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
+          const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
+          const float f = fine ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
+          uint32_t hx[4];
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const uint32_t word = q4 == 0 ? x.x : q4 == 1 ? x.y : q4 == 2 ? x.z : x.w;
+            float2 v;
+            if (kBf16)
+              v = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
+            else
+              v = __half22float2(*reinterpret_cast<const __half2*>(&word));
+            hx[q4] = fine ? h2(v.x * f, v.y * f) : 0u;
+          }
+          uint2 t8[NT];
+          terms8<NT>(hx[0], hx[1], hx[2], hx[3], t8);
+          uint8_t* const q_tile = q_tiles + (buf * C::NWG + r / RW) * C::kQBytes;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            *reinterpret_cast<uint2*>(q_tile + swz<D>(t * RW + r % RW, cl * 8)) = t8[t];
+          if (cl == 0)
+            rw.mul[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
+                             : __int_as_float(0x7fc00000);
+        }
+        ask(r0 + C::kQWarps * kPer * kBatch);
+      }
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.q_full[buf]);
     }
   } else if (warp == C::kMmaWarp) {
     if (lane == 0) {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t ring = ptx::smem_u32(smem), pb = ptx::smem_u32(p_tiles),
                      qb = ptx::smem_u32(q_tiles);
-      constexpr uint32_t idesc_s = ptx::idesc_e4m3_f32(128, C::kN);
+      // One product for the scores of all warpgroups, one for each one's values.
+      constexpr uint32_t idesc_s = ptx::idesc_e4m3_f32(128, C::NWG * C::kN);
       constexpr uint32_t idesc_o = idesc_tt(128, C::kN);
-      int n = 0, nseg = 0;
       bool ok = true;
-      auto scores = [&](bool first) {  // S^T of tile n; `first` of its item
+      auto scores = [&](int n, int k, bool first) {  // S^T of tile n, in item k
         const int i = 2 * n, st = i % NS;
-        ok = wait(&sh.kv_full[st], (i / NS) & 1);
+        if (first) ok = wait(&sh.q_full[k & 1], (k >> 1) & 1);
+        ok = ok && wait(&sh.kv_full[st], (i / NS) & 1);
+        if (n > 0) ok = ok && wait(&sh.s_free, (n - 1) & 1);
+        if (!ok) return;
+        ptx::tc_fence_after();
 #pragma unroll
-        for (int w = 0; w < C::NWG; ++w) {
-          if (first) ok = ok && wait(&sh.q_full[w], nseg & 1);
-          if (n > 0) ok = ok && wait(&sh.s_free[w], (n - 1) & 1);
-          if (!ok) return;
-          ptx::tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk)
-            ptx::umma_f8(tmem + w * 2 * C::kN,
-                         ptx::smem_desc_kmajor(ring + st * C::kSlotBytes + kk * 32, D),
-                         ptx::smem_desc_kmajor(qb + w * C::kQBytes + kk * 32, D), idesc_s,
-                         kk > 0 ? 1u : 0u);
-          ptx::umma_commit(&sh.s_full[w]);
-        }
+        for (int kk = 0; kk < D / 32; ++kk)
+          ptx::umma_f8(tmem, ptx::smem_desc_kmajor(ring + st * C::kSlotBytes + kk * 32, D),
+                       ptx::smem_desc_kmajor(qb + (k & 1) * C::NWG * C::kQBytes + kk * 32, D), idesc_s,
+                       kk > 0 ? 1u : 0u);
+        ptx::umma_commit(&sh.s_full);
         ptx::umma_commit(&sh.kv_empty[st]);
       };
-      auto values = [&](int m, bool first) {  // O^T += V^T P^T of tile m
-        const int i = 2 * m + 1, st = i % NS;
+      auto values = [&](int n, bool first) {  // O^T += V^T P^T of tile n
+        const int i = 2 * n + 1, st = i % NS;
         ok = wait(&sh.kv_full[st], (i / NS) & 1);
 #pragma unroll
         for (int w = 0; w < C::NWG; ++w) {
-          ok = ok && wait(&sh.p_full[w], m & 1);
+          ok = ok && wait(&sh.p_full[w][n & 1], (n >> 1) & 1);
           if (!ok) return;
           ptx::tc_fence_after();
+          const uint32_t p = pb + (w * C::kPBufs + n % C::kPBufs) * C::kPBytes;
 #pragma unroll
           for (int kk = 0; kk < kTileKeys / 32; ++kk)
-            ptx::umma_f8(tmem + w * 2 * C::kN + C::kN,
-                         desc_v<D>(ring + st * C::kSlotBytes + kk * 32 * D),
-                         ptx::smem_desc_mnmajor(pb + w * C::kPBytes + kk * 32 * C::kPitch, C::kPitch),
-                         idesc_o, first && kk == 0 ? 0u : 1u);
-          ptx::umma_commit(&sh.o_done[w]);
+            ptx::umma_f8(tmem + (C::NWG + w) * C::kN, desc_v<D>(ring + st * C::kSlotBytes + kk * 32 * D),
+                         ptx::smem_desc_mnmajor(p + kk * 32 * C::kPitch, C::kPitch), idesc_o,
+                         first && kk == 0 ? 0u : 1u);
+          ptx::umma_commit(&sh.o_done[w][n & 1]);
         }
         ptx::umma_commit(&sh.kv_empty[st]);
       };
-      // The scores of the next tile are issued before this tile's values, so
-      // that they are ready when the softmax of this one is done. The next
-      // item's Q is written only after this item's last values.
-      while (ok && walk.next(a, s)) {
+      // The scores of the next tile, be it the next item's first, are issued
+      // before this tile's values: they are ready when its softmax is done.
+      int n = 0, k = 0;
+      if (walk.next(a, s)) scores(0, 0, true);
+      for (bool more = true; ok && more; ++k) {
         const int count = s.t1 - s.t0;
-        scores(true);
-        for (int j = 0; ok && j < count; ++j) {
-          ++n;
-          if (j + 1 < count) scores(false);
-          if (ok) values(n - 1, j == 0);
+        for (int j = 0; ok && j < count; ++j, ++n) {
+          if (j + 1 < count) {
+            scores(n + 1, k, false);
+          } else {
+            more = walk.next(a, s);
+            if (more) scores(n + 1, k + 1, true);
+          }
+          if (ok) values(n, j == 0);
         }
-        ++nseg;
       }
       ptx::umma_commit(&sh.drain);
       wait_quietly(&sh.drain, 0, a.timeout);
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     // --------------------------------------------------------------- softmax
     const int w = warp / 4, wq = warp % 4, tid = threadIdx.x % 128;
     auto& g = sh.g[w];
-    // The warpgroup's own barrier, bounded like every other wait.
-    uint32_t met = 0;
-    auto meet = [&]() -> bool {
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sh.meet[w]);
-      return wait.warp(&sh.meet[w], met++ & 1);
-    };
-    uint8_t* const p_tile = p_tiles + w * C::kPBytes;
-    uint8_t* const q_tile = q_tiles + w * C::kQBytes;
-    const uint32_t col_s = tmem + w * 2 * C::kN + ((uint32_t)(wq * 32) << 16), col_o = col_s + C::kN;
-    int n = 0, nseg = 0;
     bool ok = true;
-    while (ok && walk.next(a, s)) {
-      ok = meet();  // the item before is done with g
-      if (!ok) break;
-      // ------------------------------------------------ rows and Q of the item
-      const int rows_seq = a.seqlen_q * a.group;
-      const int rows = rows_seq * (a.prefix_mode ? a.c.batch : 1);
-      const int row0 = s.rt * C::kRows + w * RW;
-      if (tid < RW) {
-        const int j = row0 + tid;
-        int lim = s.len, id = -1;
-        long long off = -1;
-        if (j < rows) {
-          const int b = a.prefix_mode ? j / rows_seq : s.b;
-          const int r = a.prefix_mode ? j - b * rows_seq : j;
-          const int i = r / a.group, h = s.hk * a.group + r - i * a.group;
-          int len = s.len;
-          if (a.prefix_mode) {
-            len = __ldg(a.c.seqlens + b);
-            if (len > a.c.max_len) len = 0;  // refused: its rows are not joined
-          }
-          lim = max(0, min(s.len, len - a.seqlen_q + i + 1));
-          id = (b * a.heads + h) * a.seqlen_q + i;
-          off = b * a.o_sb + h * a.o_sh + i * a.o_ss;
-        }
-        g.lim[tid] = lim;
-        g.row_id[tid] = id;
-        g.o_off[tid] = off;
-      }
-      constexpr int kLanes = D / 8;  // lanes of a row of Q
+    // The warpgroup's barrier: does any thread say yes?
+    auto any_of = [&](bool yes) -> bool {
+      uint32_t any;
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n"
+          " barrier.cta.red.or.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+          : "=r"(any)
+          : "r"(1 + w), "r"((uint32_t)yes)
+          : "memory");
+      return any != 0;
+    };
+    const uint32_t lanes = (uint32_t)(wq * 32) << 16;
+    const uint32_t col_s = tmem + w * C::kN + lanes, col_o = tmem + (C::NWG + w) * C::kN + lanes;
+    int n = 0, k = 0;
+    // A warp whose wait gave up goes on to the next barrier, and all four
+    // leave there together.
+    bool left = false;
+    for (; walk.next(a, s); ++k) {
+      const auto& rw = sh.rows[k & 1];
+      ok = ok && wait.warp(&sh.q_full[k & 1], (k >> 1) & 1);
+      const int all_see = min(rw.all_see[0], rw.all_see[1]);
+      // Rows that exist: steps without any are not computed.
+      const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
+      const int used = min(RW, rows - s.rt * C::kRows - w * RW);
+      uint64_t l2[RW / 2];  // sums of p over this thread's keys, pairs of rows
 #pragma unroll
-      for (int pass = 0; pass < (RW * kLanes + 127) / 128; ++pass) {
-        const int r = (pass * 128 + tid) / kLanes, cl = tid % kLanes;
-        const int j = row0 + r;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < RW && j < rows) {
-          const int b = a.prefix_mode ? j / rows_seq : s.b;
-          const int rr = a.prefix_mode ? j - b * rows_seq : j;
-          const int i = rr / a.group, h = s.hk * a.group + rr - i * a.group;
-          x = __ldg(reinterpret_cast<const uint4*>(
-                        a.q + 2 * (b * a.q_sb + h * a.q_sh + i * a.q_ss)) + cl);
-        }
-        uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                              __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-        m = max(m & 0xffffu, m >> 16);
-#pragma unroll
-        for (int o = kLanes / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const bool fine = m < (kBf16 ? 0x7f80u : 0x7c00u);
-        const uint32_t bits =
-            kBf16 ? m << 16
-                  : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
-        // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
-        const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
-        const float f = fine ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
-        uint32_t hx[4];
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const uint32_t word = q4 == 0 ? x.x : q4 == 1 ? x.y : q4 == 2 ? x.z : x.w;
-          float2 v;
-          if (kBf16)
-            v = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
-          else
-            v = __half22float2(*reinterpret_cast<const __half2*>(&word));
-          hx[q4] = fine ? h2(v.x * f, v.y * f) : 0u;
-        }
-        uint2 t8[NT];
-        terms8<NT>(hx[0], hx[1], hx[2], hx[3], t8);
-        if (r < RW) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            *reinterpret_cast<uint2*>(q_tile + swz<D>(t * RW + r, cl * 8)) = t8[t];
-          if (cl == 0)
-            g.mul[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
-                            : __int_as_float(0x7fc00000);
-        }
-      }
-      ptx::fence_proxy_async_smem();
-      ok = meet();  // mul, lim and row_id are there for all
-      if (!ok) break;
-      if (lane == 0) ptx::mbar_arrive(&sh.q_full[w]);
-      int all_see = s.len;  // keys that every row sees
-#pragma unroll
-      for (int r = 0; r < RW; ++r) all_see = min(all_see, g.lim[r]);
-
-      const int* table = a.c.table + (a.prefix_mode ? 0 : s.b) * a.c.table_stride;
-      const uint8_t* ke = a.c.k_exp + s.hk * a.c.ke_sh;
-      const uint8_t* ve = a.c.v_exp + s.hk * a.c.ve_sh;
-      // Page of this thread's key in tile t, and the key's exponent bytes
-      // (K in the low half): both asked for one tile before they are needed.
-      auto page_at = [&](int t) {
-        const int key = a.key_base + t * kTileKeys + tid;
-        return key < s.len && t < s.t1 ? __ldg(table + page_of(a, key)) : 0;
-      };
-      auto bytes_at = [&](int t, int page) -> uint32_t {
-        const int key = a.key_base + t * kTileKeys + tid;
-        if (key >= s.len || key < a.key0 || t >= s.t1) return 127u | (127u << 16);
-        if (page < 0 || page >= a.c.num_pages) {
-          if (a.c.status) atomicOr(a.c.status, FA8_DEVERR_PAGE_RANGE);
-          return 255u | (255u << 16);
-        }
-        const int slot = key - page_of(a, key) * a.c.page_size;
-        return (uint32_t)__ldg(ke + page * a.c.ke_sp + slot) |
-               ((uint32_t)__ldg(ve + page * a.c.ve_sp + slot) << 16);
-      };
-      uint32_t eb_next = bytes_at(s.t0, page_at(s.t0));
-      int page_next = page_at(s.t0 + 1);
-
-      float m[RW], l[RW];
-      float m_lane = -INFINITY;  // running maximum of row `lane`
-#pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        m[r] = 0.f;
-        l[r] = 0.f;
-      }
+      for (int r = 0; r < RW / 2; ++r) l2[r] = 0;
+      // Running maximum of row `lane`. A row that sees any of this block's keys
+      // of the item sees some of the first tile: that one sets it.
+      float m_lane = 0.f;
+      if (lane < RW) g.neg_m[lane] = 0.f;  // (every warp writes the same)
+      __syncwarp();
       for (int t = s.t0; t < s.t1; ++t, ++n) {
-        const uint32_t eb = eb_next;
-        eb_next = bytes_at(t + 1, page_next);
-        page_next = page_at(t + 2);
-        const int key = a.key_base + t * kTileKeys + tid;
-        const float kf = kv::exp_factor((int)(eb & 0xffffu));
-        const int vb = (int)(eb >> 16);
-        const float vexp = vb == kv::kExpNan ? 0.f : (float)(vb - kv::kExpBias);
-        const float vf = kv::exp_factor(vb) * kPScale;
-        // Every key of the tile seen by every row?
-        const int first_key = a.key_base + t * kTileKeys;
+        const int first_key = a.key_base + t * kTileKeys, key = first_key + tid;
+        // Every key of the tile seen by every row? This one by any?
         const bool plain = first_key >= a.key0 && first_key + kTileKeys <= all_see;
+        const bool dead = key < a.key0 || key >= s.len;
+        ok = ok && wait.warp(&sh.e_full[n % kExpTiles], (n / kExpTiles) & 1);
+        const int kb = sh.exps[n % kExpTiles][0][tid], vb = sh.exps[n % kExpTiles][1][tid];
+        const float kf = kv::exp_factor(kb);
+        const float vexp = vb == kv::kExpNan ? 0.f : (float)(vb - kv::kExpBias);
+        const float vf = dead ? 0.f : kv::exp_factor(vb) * kPScale;
 
-        ok = wait.warp(&sh.s_full[w], n & 1);
-        if (!ok) break;
+        ok = ok && wait.warp(&sh.s_full, n & 1);
         ptx::tc_fence_after();
-        float x[RW];
-        {
-          uint32_t raw[NT * RW];
+        uint64_t d2[RW / 2];  // scores in base 2 above the running maximum
+        float high = -INFINITY;
+        const uint64_t kf2 = ptx::pack2(kf, kf);
 #pragma unroll
-          for (int q = 0; q < NT; ++q) tmem_ld<RW>(col_s + q * RW, raw + q * RW);
-          wait_ld<NT * RW>(raw);
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(&sh.s_free[w]);
+        for (int c = 0; c < RW; c += C::kStep) {
+          if (c < used) {
+            constexpr int K = C::kStep;
+            uint32_t raw[NT * K];
 #pragma unroll
-          for (int r = 0; r < RW; ++r) {
-            float v = __uint_as_float(raw[(NT - 1) * RW + r]);
+            for (int q = 0; q < NT; ++q) tmem_ld<K>(col_s + q * RW + c, raw + q * K);
+            wait_ld<NT * K>(raw);
+            const uint64_t inv2 = ptx::pack2(1.f / kTerm, 1.f / kTerm);
 #pragma unroll
-            for (int q = NT - 2; q >= 0; --q)
-              v = fmaf(v, 1.f / kTerm, __uint_as_float(raw[q * RW + r]));
-            x[r] = v * (kf * g.mul[r]);
+            for (int r = 0; r < K; r += 4) {
+              const ulonglong2 mul = *reinterpret_cast<const ulonglong2*>(&rw.mul[w * RW + c + r]);
+              const ulonglong2 nm = *reinterpret_cast<const ulonglong2*>(&g.neg_m[c + r]);
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                auto pair = [&](int q) {
+                  return ptx::pack2(__uint_as_float(raw[q * K + r + e]),
+                                    __uint_as_float(raw[q * K + r + e + 1]));
+                };
+                uint64_t v = pair(NT - 1);
+#pragma unroll
+                for (int q = NT - 2; q >= 0; --q) v = ptx::ffma2(v, inv2, pair(q));
+                d2[(c + r + e) / 2] =
+                    ptx::ffma2(v, ptx::fmul2(kf2, e ? mul.y : mul.x), e ? nm.y : nm.x);
+              }
+            }
           }
         }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sh.s_free);
         if (!plain) {
 #pragma unroll
-          for (int r = 0; r < RW; ++r)
-            if (key < a.key0 || key >= g.lim[r]) x[r] = -INFINITY;
-        }
-        // Largest s + e of each row over the tile, against the running one.
-        float top = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-          const float v = warp_max(x[r] + vexp);
-          if (lane == r) top = v;
-        }
-        if (lane < RW) g.top[n & 1][wq][lane] = top;
-        ok = meet();
-        if (!ok) break;
-        float f_lane = 1.f;
-        bool up = false;
-        if (lane < RW) {
-          const float v = fmaxf(fmaxf(g.top[n & 1][0][lane], g.top[n & 1][1][lane]),
-                                fmaxf(g.top[n & 1][2][lane], g.top[n & 1][3][lane]));
-          up = v > m_lane + kRise;
-          if (up) {
-            f_lane = m_lane == -INFINITY ? 0.f : ptx::ex2(m_lane - v);
-            m_lane = v;
+          for (int r = 0; r < RW; r += 2) {
+            float d0, d1;
+            ptx::unpack2(d2[r / 2], d0, d1);
+            if (dead || key >= rw.lim[w * RW + r]) d0 = -INFINITY;
+            if (dead || key >= rw.lim[w * RW + r + 1]) d1 = -INFINITY;
+            d2[r / 2] = ptx::pack2(d0, d1);
           }
         }
-        // The values of the tile before are complete: P may be overwritten and
-        // O rescaled.
-        const bool any_up = __any_sync(0xffffffffu, up);
-        if (n > 0) {
-          ok = wait.warp(&sh.o_done[w], (n - 1) & 1);
-          if (!ok) break;
+#pragma unroll
+        for (int r = 0; r < RW; r += 2) {
+          if (r / C::kStep * C::kStep < used) {
+            float d0, d1;
+            ptx::unpack2(d2[r / 2], d0, d1);
+            high = ptx::fmax3(high, d0, d1);
+          }
         }
-        if (any_up) {
+
+        // Does a row rise above its maximum by more than kRise? Then the
+        // largest s + e of each row over the tile is its new one.
+        const bool rise = any_of(t == s.t0 || high + vexp > kRise || !ok);
+        // P's buffer is free: the product that read it two tiles ago was
+        // issued before these scores, whose completion covers it. With one
+        // buffer the product of the tile before has to be waited for.
+        if (C::kPBufs == 1 && n > 0) ok = ok && wait.warp(&sh.o_done[w][(n - 1) & 1], ((n - 1) >> 1) & 1);
+        if (rise) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < RW; r += 2) {
+            if (r / C::kStep * C::kStep < used) {
+              float d0, d1;
+              ptx::unpack2(d2[r / 2], d0, d1);
+              d0 = warp_max(d0 + vexp);
+              d1 = warp_max(d1 + vexp);
+              if (lane == r) top = d0;
+              if (lane == r + 1) top = d1;
+            }
+          }
+          if (lane < RW) reinterpret_cast<float*>(&g.top[lane])[wq] = top;
+          if (any_of(!ok)) {
+            left = true;
+            break;
+          }
+          float f_lane = 1.f;
+          if (lane < RW) {
+            const float4 v4 = g.top[lane];
+            const float v = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
+            float by = 0.f;
+            if (v > (t == s.t0 ? -INFINITY : kRise)) {
+              by = v;
+              f_lane = t == s.t0 ? 0.f : ptx::ex2(-v);
+              m_lane += v;
+            }
+            g.step[lane] = -by;
+            g.neg_m[lane] = -m_lane;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < RW; r += 4) {
+            if (r / C::kStep * C::kStep < used) {
+              const ulonglong2 by = *reinterpret_cast<const ulonglong2*>(&g.step[r]);
+              d2[r / 2] = ptx::fadd2(d2[r / 2], by.x);
+              d2[r / 2 + 1] = ptx::fadd2(d2[r / 2 + 1], by.y);
+            }
+          }
           if (t > s.t0) {
+            // The sums so far, rescaled; O when the tile before is in it.
+            const uint32_t rose = __ballot_sync(0xffffffffu, f_lane != 1.f);
+            ok = ok && wait.warp(&sh.o_done[w][(n - 1) & 1], ((n - 1) >> 1) & 1);
             ptx::tc_fence_after();
 #pragma unroll
-            for (int q = 0; q < NT; ++q) {
+            for (int c = 0; c < RW; c += 8) {
+              if ((rose >> c) & 0xffu) {
+                uint32_t o8[NT * 8];
 #pragma unroll
-              for (int c = 0; c < RW; c += 8) {
-                uint32_t o8[8];
-                tmem_ld<8>(col_o + q * RW + c, o8);
-                wait_ld<8>(o8);
+                for (int q = 0; q < NT; ++q) tmem_ld<8>(col_o + q * RW + c, o8 + q * 8);
+                wait_ld<NT * 8>(o8);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  o8[k] = __float_as_uint(__uint_as_float(o8[k]) *
-                                          __shfl_sync(0xffffffffu, f_lane, c + k));
-                tmem_st8(col_o + q * RW + c, o8);
+                for (int r = 0; r < 8; r += 2) {
+                  const float f0 = __shfl_sync(0xffffffffu, f_lane, c + r);
+                  const float f1 = __shfl_sync(0xffffffffu, f_lane, c + r + 1);
+                  l2[(c + r) / 2] = ptx::fmul2(l2[(c + r) / 2], ptx::pack2(f0, f1));
+#pragma unroll
+                  for (int q = 0; q < NT; ++q) {
+                    o8[q * 8 + r] = __float_as_uint(__uint_as_float(o8[q * 8 + r]) * f0);
+                    o8[q * 8 + r + 1] = __float_as_uint(__uint_as_float(o8[q * 8 + r + 1]) * f1);
+                  }
+                }
+#pragma unroll
+                for (int q = 0; q < NT; ++q) tmem_st8(col_o + q * RW + c, o8 + q * 8);
               }
             }
             ptx::tmem_wait_st();
           }
-          const float use = m_lane == -INFINITY ? 0.f : m_lane;
+        }
+        // p, its sum, and the key's row of P: the terms side by side. A key
+        // that some rows do not see may have a NaN factor: their product with
+        // it is then not formed (kPick).
+        uint8_t* const p_tile = p_tiles + (w * C::kPBufs + n % C::kPBufs) * C::kPBytes;
+        auto emit = [&](auto pick) {
+          constexpr bool kPick = decltype(pick)::value;
+          const uint64_t vf2 = ptx::pack2(vf, vf);
 #pragma unroll
-          for (int r = 0; r < RW; ++r) {
-            l[r] *= __shfl_sync(0xffffffffu, f_lane, r);
-            m[r] = __shfl_sync(0xffffffffu, use, r);
+          for (int c = 0; c < RW; c += 8) {
+            if (c < used) {
+              uint32_t y[4];
+#pragma unroll
+              for (int r = 0; r < 8; r += 2) {
+                float d0, d1, y0, y1;
+                ptx::unpack2(d2[(c + r) / 2], d0, d1);
+                const uint64_t p = ptx::pack2(ptx::ex2(d0), ptx::ex2(d1));
+                l2[(c + r) / 2] = ptx::fadd2(l2[(c + r) / 2], p);
+                ptx::unpack2(ptx::fmul2(p, vf2), y0, y1);
+                if (kPick && d0 == -INFINITY) y0 = 0.f;
+                if (kPick && d1 == -INFINITY) y1 = 0.f;
+                y[r / 2] = h2(y0, y1);
+              }
+              uint2 t8[NT];
+              terms8<NT>(y[0], y[1], y[2], y[3], t8);
+#pragma unroll
+              for (int q = 0; q < NT; ++q)
+                *reinterpret_cast<uint2*>(p_tile + swz<C::kPitch>(tid, q * RW + c)) = t8[q];
+            }
           }
-        }
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-          const float p = ptx::ex2(x[r] - m[r]);
-          l[r] += p;
-          // A masked key's factor may be anything: its product is not formed.
-          x[r] = !plain && x[r] == -INFINITY ? 0.f : p * vf;
-        }
-        // The key's row of P: the terms side by side.
-#pragma unroll
-        for (int c = 0; c < RW; c += 8) {
-          uint2 t8[NT];
-          terms8<NT>(h2(x[c], x[c + 1]), h2(x[c + 2], x[c + 3]), h2(x[c + 4], x[c + 5]),
-                     h2(x[c + 6], x[c + 7]), t8);
-#pragma unroll
-          for (int q = 0; q < NT; ++q)
-            *reinterpret_cast<uint2*>(p_tile + swz<C::kPitch>(tid, q * RW + c)) = t8[q];
-        }
+        };
+        if (!plain && __any_sync(0xffffffffu, vb == kv::kExpNan))
+          emit(std::true_type());
+        else
+          emit(std::false_type());
         // Rows of V that are not this item's keys (the end of a page, a page
         // not brought in) may hold anything, NaN codes among them: zeros.
         if (w == 0 && (first_key < a.key0 || first_key + kTileKeys > s.len)) {
           const int st = (2 * n + 1) % NS;
-          ok = wait.warp(&sh.kv_full[st], ((2 * n + 1) / NS) & 1);
-          if (!ok) break;
-          if (key < a.key0 || key >= s.len) {
+          ok = ok && wait.warp(&sh.kv_full[st], ((2 * n + 1) / NS) & 1);
+          if (dead) {
             uint4* row = reinterpret_cast<uint4*>(smem + st * C::kSlotBytes + tid * D);
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) row[c] = make_uint4(0, 0, 0, 0);
@@ -835,91 +1021,86 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&sh.p_full[w]);
+        if (lane == 0) ptx::mbar_arrive(&sh.p_full[w][n & 1]);
       }
-      if (!ok) break;
+      if (left) break;
 
       // ------------------------------------------------------ the item's result
+      {
+        float l[RW];
 #pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        float v = l[r];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == r) g.sum[wq][r] = v;
+        for (int r = 0; r < RW; r += 2) ptx::unpack2(l2[r / 2], l[r], l[r + 1]);
+        const float v = warp_sums<RW>(l);
+        constexpr int kEach = 32 / RW;  // lanes that hold the same row's sum
+        if (lane % kEach == 0) reinterpret_cast<float*>(&g.sum[lane / kEach])[wq] = v;
       }
-      ok = wait.warp(&sh.o_done[w], (n - 1) & 1);
-      if (!ok) break;
+      ok = ok && wait.warp(&sh.o_done[w][(n - 1) & 1], ((n - 1) >> 1) & 1);
       ptx::tc_fence_after();
-      ok = meet();
-      if (!ok) break;
+      if (any_of(!ok)) break;
       const bool begins = s.t0 == 0, whole = begins && s.t1 == s.nt;
-      const int part = 2 * cta + (nseg > 0 ? 1 : 0);
-      if (tid < RW) {
-        const float sum = (g.sum[0][tid] + g.sum[1][tid]) + (g.sum[2][tid] + g.sum[3][tid]);
-        // Row `tid` is row `lane` of warp 0, whose lanes hold the maxima.
-        const float top = sum == 0.f ? -INFINITY : (m_lane == -INFINITY ? 0.f : m_lane);
-        const int id = g.row_id[tid];
-        if (!whole) {
-          a.part_ml[(long long)part * C::kRows + w * RW + tid] = make_float2(top, sum);
-        } else if (!a.own_rows) {
-          if (id >= 0) a.full_ml[id] = make_float2(top, sum);
-        } else {
-          g.inv[tid] = sum == 0.f ? 0.f : 1.f / (kPScale * sum);
-          if (id >= 0 && a.lse)
-            a.lse[id] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+      const int part = 2 * cta + (k > 0 ? 1 : 0);
+      // Lane r looks after row r (its maximum is there).
+      float inv_lane = 0.f;
+      int id_lane = -1;
+      if (lane < used) {
+        id_lane = rw.row_id[w * RW + lane];
+        const float sum = sum_of(g.sum[lane]);
+        const float top = sum == 0.f ? -INFINITY : m_lane;
+        inv_lane = sum == 0.f ? 0.f : __fdividef(1.f / kPScale, sum);
+        if (wq == 0) {
+          if (!whole)
+            a.part_ml[(long long)part * C::kRows + w * RW + lane] = make_float2(top, sum);
+          else if (!a.own_rows)
+            a.full_ml[id_lane] = make_float2(top, sum);
+          else if (a.lse)
+            a.lse[id_lane] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
         }
       }
-      if (w == 0 && tid == 0) {
-        // Block that holds the item's last tile: the last c with U c / G < unit + 1.
-        auto last_block = [&](long long unit) {
-          return (int)(((unit + 1) * shares - 1) / total);
-        };
-        if (a.own_rows) {
-          if (begins && !whole)
-            a.seg[cta] = make_int4(last_block(s.unit + s.nt - 1), s.b,
-                                   s.hk * a.row_tiles + s.rt, part);
-        } else if (begins) {
+      if (w == 0 && tid == 0 && begins && !(a.own_rows && whole)) {
+        // Says where the item's parts are: from this block to its last tile's.
+        const int last = whole ? cta : shares.block_of(s.unit + s.nt - 1);
+        if (a.own_rows)
+          a.seg[cta] = make_int4(last, s.b, s.hk * a.row_tiles + s.rt, part);
+        else
           a.item[(long long)s.b * per + s.hk * a.row_tiles + s.rt] =
-              make_int4(cta, whole ? cta : last_block(s.unit + s.nt - 1), part,
-                        whole ? kItemFull : kItemParts);
-        }
+              make_int4(cta, last, part, whole ? kItemFull : kItemParts);
       }
-      ok = meet();
-      if (!ok) break;
       // O^T: a thread has one d of every row; with D = 64 the upper half of the
       // lanes repeats the lower and takes the odd rows.
       const int d = tid % D;
-      const bool own_half = D == 128;
 #pragma unroll
       for (int c = 0; c < RW; c += 8) {
-        uint32_t raw[NT * 8];
+        if (c < used) {
+          uint32_t raw[NT * 8];
 #pragma unroll
-        for (int q = 0; q < NT; ++q) tmem_ld<8>(col_o + q * RW + c, raw + q * 8);
-        wait_ld<NT * 8>(raw);
+          for (int q = 0; q < NT; ++q) tmem_ld<8>(col_o + q * RW + c, raw + q * 8);
+          wait_ld<NT * 8>(raw);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          float v = __uint_as_float(raw[(NT - 1) * 8 + k]);
+          for (int e = 0; e < 8; ++e) {
+            const int r = c + e;
+            const float inv = __shfl_sync(0xffffffffu, inv_lane, r);
+            const long long to =
+                whole ? rw.off[w * RW + r] : ((long long)part * C::kRows + w * RW + r) * D;
+            float v = __uint_as_float(raw[(NT - 1) * 8 + e]);
 #pragma unroll
-          for (int q = NT - 2; q >= 0; --q)
-            v = fmaf(v, 1.f / kTerm, __uint_as_float(raw[q * 8 + k]));
-          const int r = c + k;
-          const int id = g.row_id[r];
-          if (id < 0 || !(own_half || (r & 1) == tid / 64)) continue;
-          if (!whole) {
-            a.part_o[((long long)part * C::kRows + w * RW + r) * D + d] = v;
-          } else if (!a.own_rows) {
-            a.full_o[(long long)id * D + d] = v;
-          } else {
-            const float y = v * g.inv[r];
-            if (kBf16)
-              reinterpret_cast<__nv_bfloat16*>(a.o)[g.o_off[r] + d] = __float2bfloat16(y);
-            else
-              reinterpret_cast<__half*>(a.o)[g.o_off[r] + d] = __float2half(y);
+            for (int q = NT - 2; q >= 0; --q)
+              v = fmaf(v, 1.f / kTerm, __uint_as_float(raw[q * 8 + e]));
+            if (r < used && (D == 128 || (r & 1) == tid / 64)) {
+              if (!whole)
+                a.part_o[to + d] = v;
+              else if (!a.own_rows)
+                a.full_o[to + d] = v;
+              else if (kBf16)
+                reinterpret_cast<__nv_bfloat16*>(a.o)[to + d] = __float2bfloat16(v * inv);
+              else
+                reinterpret_cast<__half*>(a.o)[to + d] = __float2half(v * inv);
+            }
           }
         }
       }
       ptx::tc_fence_before();
-      ++nseg;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.q_free[k & 1]);
     }
   }
 
@@ -976,13 +1157,20 @@ struct RowSum {
 #pragma unroll
       for (int e = 0; e < V; ++e) o[e] *= keep;
       m = top;
-#pragma unroll 4
-      for (int i = 0; i < here; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, i);
-        float x[V];
-        load(po + at(i0 + i) * D + lane * V, x);
+      // The rows come in sixteens that are all on their way at once; behind
+      // the last one it is read again, with no weight.
+      constexpr int kFly = 16;
+#pragma unroll 1
+      for (int i = 0; i < here; i += kFly) {
+        float x[kFly][V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(wi, x[e], o[e]);
+        for (int u = 0; u < kFly; ++u) load(po + at(i0 + min(i + u, here - 1)) * D + lane * V, x[u]);
+#pragma unroll
+        for (int u = 0; u < kFly; ++u) {
+          const float wi = __shfl_sync(0xffffffffu, w, min(i + u, here - 1));
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[e] = fmaf(i + u < here ? wi : 0.f, x[u][e], o[e]);
+        }
       }
     }
   }
@@ -1012,9 +1200,11 @@ struct RowSum {
 };
 
 // Joins the parts of the item that block `blockIdx.x` of the first kernel
-// began and did not end; a warp per row.
+// began and did not end; a warp per row. The bound of four blocks an SM lets
+// the compiler hold a batch of rows in registers: without it it took 32 and
+// waited for each row by itself (75 parts: 13 us).
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) decode_join_kernel(const Args a, int tile_rows) {
+__global__ void __launch_bounds__(128, 4) decode_join_kernel(const Args a, int tile_rows) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 s = __ldcg(a.seg + blockIdx.x);  // last block, sequence, head and row tile, part
   if (s.x < 0) return;
@@ -1041,7 +1231,7 @@ struct Set {
 
 // Joins every row's prefix with what is behind it; a warp per row.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) prefix_join_kernel(const Args a, const Set pre, const Set own) {
+__global__ void __launch_bounds__(128, 4) prefix_join_kernel(const Args a, const Set pre, const Set own) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int id = blockIdx.x * 4 + threadIdx.x / 32;
   if (id >= a.c.batch * a.heads * a.seqlen_q) return;
@@ -1085,6 +1275,14 @@ int check(const fa8_decode_params* p, bool* empty) {
     return fa8_note_error(FA8_ERR_UNSUPPORTED, "fa8_decode: too many query rows");
   if (p->prefix_len > p->cache.max_pages * p->cache.page_size)
     return fa8_note_error(FA8_ERR_INVALID_ARG, "fa8_decode: prefix_len does not fit the page table");
+  // Key tiles of all items number less than 2^31, whatever the lengths are.
+  const int64_t group = p->heads / p->cache.heads_kv;
+  const int64_t tiles = (p->cache.max_pages * p->cache.page_size + 2 * kTileKeys - 1) / kTileKeys;
+  for (int64_t rows : {p->seqlen_q * group, p->seqlen_q * group * p->cache.batch}) {
+    const int64_t seqs = rows == p->seqlen_q * group ? p->cache.batch : 1;
+    if (seqs * p->cache.heads_kv * ((rows + 7) / 8) > (1ll << 31) / tiles - 1)
+      return fa8_note_error(FA8_ERR_UNSUPPORTED, "fa8_decode: too many key tiles for one call");
+  }
   if (!(p->softmax_scale > 0.f) || !std::isfinite(p->softmax_scale))
     return fa8_note_error(FA8_ERR_INVALID_ARG, "fa8_decode: softmax_scale must be positive and finite");
   if (!p->q || !p->o) return fa8_note_error(FA8_ERR_INVALID_ARG, "fa8_decode: null q or o");
@@ -1151,7 +1349,7 @@ Shape shape_for(int64_t rows) {
   if (rows <= 32) return {32, 1};
   return {32, 2};
 }
-int ctas_per_sm(int64_t d, const Shape& s) { return s.nwg > 1 ? 1 : (d == 64 && s.rw <= 16 ? 3 : 2); }
+int ctas_per_sm(int64_t d, const Shape& s) { return s.nwg > 1 ? 1 : (d == 64 && s.rw == 8 ? 3 : 2); }
 
 constexpr int kSmCount = 148;
 
@@ -1211,8 +1409,13 @@ int launch_set(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, int 
   auto kernel = decode_kernel<C, kBf16>;
   std::call_once(flags[dev], [&] {
     errs[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    cudaFuncAttributes at;
+    if (errs[dev] == cudaSuccess) errs[dev] = cudaFuncGetAttributes(&at, kernel);
+    // The register split draws on what the block is launched with.
+    if (errs[dev] == cudaSuccess && at.numRegs != C::kRegsLaunch)
+      errs[dev] = cudaErrorInvalidKernelImage;
   });
-  if (errs[dev] != cudaSuccess) return fa8_note_cuda_error(errs[dev], "cudaFuncSetAttribute");
+  if (errs[dev] != cudaSuccess) return fa8_note_cuda_error(errs[dev], "decode kernel attributes");
   const cudaError_t e = launch_early(kernel, dim3((unsigned)grid), C::kThreads, C::kSmem, stream,
                                      a.early != 0, tk, tv, a);
   return e == cudaSuccess ? FA8_OK : fa8_note_cuda_error(e, "decode kernel launch");
@@ -1346,9 +1549,8 @@ int fa8_decode(const fa8_decode_params* p, void* workspace, int64_t workspace_by
   a.prefix_len = (int)p->prefix_len;
   const int page = (int)p->cache.page_size;
   a.box = std::min(page, kTileKeys);
-  a.page_shift = -1;
-  for (int s = 0; s < 31; ++s)
-    if (page == 1 << s) a.page_shift = s;
+  while ((1 << a.page_shift) < page) ++a.page_shift;
+  a.page_mul = (uint32_t)((((1ull << a.page_shift) - page) << 32) / page + 1);
   a.q_sb = p->q_stride_b;
   a.q_sh = p->q_stride_h;
   a.q_ss = p->q_stride_s;

@@ -58,6 +58,11 @@ int check_cache(const fa8_kv_cache& c) {
   for (int64_t s : {c.k_exp_stride_p, c.k_exp_stride_h, c.v_exp_stride_p, c.v_exp_stride_h})
     if (s <= 0)
       return fa8_note_error(FA8_ERR_INVALID_ARG, "cache: exponent strides must be positive");
+  // The attention reads them 16 at a time.
+  if (((reinterpret_cast<uintptr_t>(c.k_exp) | reinterpret_cast<uintptr_t>(c.v_exp)) & 15) ||
+      ((c.k_exp_stride_p | c.k_exp_stride_h | c.v_exp_stride_p | c.v_exp_stride_h) & 15))
+    return fa8_note_error(FA8_ERR_ALIGNMENT,
+                          "cache: exponents must be 16-byte aligned, their strides multiples of 16");
   return FA8_OK;
 }
 

@@ -90,6 +90,8 @@ CACHE_REFUSALS = [
     (_set(c_v_stride_p=0), "FA8_ERR_ALIGNMENT"),
     (_set(c_k_stride_s=64), "FA8_ERR_INVALID_ARG"),
     (_set(c_v_exp_stride_h=0), "FA8_ERR_INVALID_ARG"),
+    (_set(c_k_exp=0x100008), "FA8_ERR_ALIGNMENT"),
+    (_set(c_v_exp_stride_p=72), "FA8_ERR_ALIGNMENT"),
 ]
 
 
@@ -119,6 +121,7 @@ def test_copy_refusals(abi, call, mutate, status):
     (_set(seqlen_q=65536), "FA8_ERR_UNSUPPORTED"),
     (_set(prefix_len=-1), "FA8_ERR_INVALID_ARG"),
     (_set(prefix_len=81), "FA8_ERR_INVALID_ARG"),
+    (_set(c_max_pages=1 << 25, c_batch=4096), "FA8_ERR_UNSUPPORTED"),  # 2^31 key tiles
     (_set(softmax_scale=0.0), "FA8_ERR_INVALID_ARG"),
     (_set(softmax_scale=math.inf), "FA8_ERR_INVALID_ARG"),
     (_set(dtype=3), "FA8_ERR_INVALID_ARG"),
