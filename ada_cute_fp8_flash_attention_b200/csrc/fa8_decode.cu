@@ -83,15 +83,19 @@ struct Cfg {
   static constexpr int kMmaWarp = NWG * 4, kLoadWarp = NWG * 4 + 1, kQWarp = NWG * 4 + 2;
   static constexpr int kQWarps = 2;
   static constexpr int kN = (NT * RW + 15) / 16 * 16;  // columns of the products
-  static constexpr int kStep = RW < 16 ? 8 : 16;       // rows read from TMEM at a time
-  static constexpr int kPitch = kN <= 64 ? 64 : 128;   // bytes of a key's row of P
+  static constexpr int kStep = NWG == 1 ? RW : 8;     // rows read from TMEM at a time
+  // P of all warpgroups side by side: bytes of a key's row, in atoms of up to
+  // 128 (three terms of 64 rows take one and a half).
+  static constexpr int kPCols = NWG * kN;
+  static constexpr int kPitch = kPCols <= 32 ? 32 : kPCols <= 64 ? 64 : 128;
+  static constexpr int kPAtoms = (kPCols + kPitch - 1) / kPitch;
   static constexpr int kSlotBytes = kTileKeys * D;     // a K or a V tile
   static constexpr int kQBytes = kN * D;               // per warpgroup
-  static constexpr int kPBytes = kTileKeys * kPitch;
+  static constexpr int kPBytes = kTileKeys * kPitch * kPAtoms;
   static constexpr uint32_t kTmemUsed = 2u * kN * NWG;
   static constexpr uint32_t kTmemCols =
       kTmemUsed <= 32 ? 32 : kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
-  static constexpr int kCtas = NWG > 1 ? 1 : (D == 64 && RW == 8 ? 3 : 2);  // per SM
+  static constexpr int kCtas = NWG > 2 ? 1 : (D == 64 && RW == 8 ? 3 : 2);  // per SM
   // 227 KB a block, 228 KB an SM of which each block takes 1 KB and its
   // static variables; 1 KB to align.
   static constexpr int kStatic = 2688 + 80 * kRows;
@@ -99,23 +103,38 @@ struct Cfg {
   // P in two buffers where four tiles of the ring still fit beside them: the
   // next one is then written while the product of this one runs.
   static constexpr int slots_with(int bufs) {
-    const int n = (kBudget - NWG * (2 * kQBytes + bufs * kPBytes)) / kSlotBytes;
+    const int n = (kBudget - NWG * 2 * kQBytes - bufs * kPBytes) / kSlotBytes;
     return n < 12 ? n : 12;
   }
   static constexpr int kPBufs = slots_with(2) >= 4 ? 2 : 1;
   static constexpr int kSlots = slots_with(kPBufs);
-  static constexpr int kSmem = kSlots * kSlotBytes + NWG * (2 * kQBytes + kPBufs * kPBytes) + 1024;
+  static constexpr int kSmem = kSlots * kSlotBytes + NWG * 2 * kQBytes + kPBufs * kPBytes + 1024;
   // Registers: what the launch bounds give a thread, moved from the helpers
   // (loads, products, Q) to the softmax warpgroups.
   static constexpr int kRegsLaunch = 65536 / (kCtas * kThreads) / 8 * 8;
-  static constexpr int kRegsHelp = kCtas == 3 ? 56 : (NWG > 1 ? 88 : 72);
+  static constexpr int kRegsHelp = NWG == 1 && kCtas == 2 ? 80 : 64;
   static constexpr int kRegsSoft = ((NWG + 1) * kRegsLaunch - kRegsHelp) / NWG / 8 * 8;
   static_assert(NWG * kRegsSoft + kRegsHelp <= (NWG + 1) * kRegsLaunch && kRegsSoft <= 255,
                 "setmaxnreg must not ask for more than the block was launched with");
   static_assert(kTmemUsed <= 512 && kTmemCols * kCtas <= 512, "TMEM of the resident blocks");
   static_assert(kSlots >= 4, "a K and a V tile in use and two on their way");
-  static_assert(RW == 8 || RW == 16 || RW == 32, "rows of a warpgroup");
+  static_assert(RW == 8 || RW == 16, "rows of a warpgroup");
   static_assert(kN <= 128 && kSlotBytes % 1024 == 0 && kPBytes % 1024 == 0, "tile alignment");
+};
+
+// x / d for 0 <= x < 2^31 by one multiplication.
+struct Divisor {
+  uint32_t mul, shift;
+  int d;
+  static Divisor of(int d) {
+    Divisor v{0, 0, d};
+    while ((1ll << v.shift) < d) ++v.shift;
+    v.mul = (uint32_t)((((1ull << v.shift) - d) << 32) / d + 1);
+    return v;
+  }
+  __device__ __forceinline__ int div(int x) const {
+    return (int)((__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
+  }
 };
 
 struct Args {
@@ -131,7 +150,7 @@ struct Args {
   int prefix_len;
   int row_tiles;     // tiles of query rows per (sequence, K/V head)
   int box;           // keys of a TMA box: min(page_size, 128)
-  uint32_t page_mul, page_shift;  // key / page_size = (mulhi(key, mul) + key) >> shift
+  Divisor by_page, by_group, by_seq_rows, by_row_tiles;  // page_size, group, group * seqlen_q, row_tiles
   int own_rows;      // results go to o (1), or to full_* and item (0)
   int early;         // this launch may overlap the one before it
   float scale_log2;
@@ -218,11 +237,11 @@ __device__ __forceinline__ void terms8(uint32_t x0, uint32_t x1, uint32_t x2, ui
   }
 }
 // Byte offset of column byte `col` of row `row` in a tile of rows of kPitch
-// bytes under the 64 B or 128 B swizzle.
+// bytes under the 32 B, 64 B or 128 B swizzle.
 template <int kPitch>
 __device__ __forceinline__ uint32_t swz(int row, int col) {
   const int chunk = col >> 4;
-  const int x = kPitch == 128 ? (row & 7) : ((row >> 1) & 3);
+  const int x = kPitch == 128 ? (row & 7) : kPitch == 64 ? ((row >> 1) & 3) : ((row >> 2) & 1);
   return (uint32_t)(row * kPitch + ((chunk ^ x) << 4) + (col & 15));
 }
 
@@ -241,6 +260,15 @@ __device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
 }
 
 __device__ __forceinline__ float sum_of(const float4& v) { return (v.x + v.y) + (v.z + v.w); }
+
+// P^T as operand B: rows (keys) of kPitch bytes; columns beyond them are in the
+// next atom, a whole tile further on.
+template <int kPitch>
+__device__ __forceinline__ uint64_t desc_p(uint32_t addr) {
+  uint64_t d = ptx::smem_desc_mnmajor(addr, kPitch);
+  if (kPitch == 32) d = (d & ~(7ull << 61)) | (6ull << 61);  // SWIZZLE_32B
+  return (d & ~(0x3FFFull << 16)) | ((uint64_t)(kTileKeys * kPitch >> 4) << 16);
+}
 
 // -------------------------------------------------------------------- waiting
 // Every wait is bounded. One that gave up sets the block's abort flag, which
@@ -343,7 +371,7 @@ struct Shares {
 };
 
 __device__ __forceinline__ int page_of(const Args& a, int key) {
-  return (int)((__umulhi((uint32_t)key, a.page_mul) + (uint32_t)key) >> a.page_shift);
+  return a.by_page.div(key);
 }
 
 constexpr int kExpTiles = 8;  // ring of exponent bytes: tiles in flight and two more
@@ -361,8 +389,8 @@ struct __align__(16) Shared {
   // P^T in shared memory (and O^T rescaled), tiles in turn: the softmax may be
   // done with tile n + 1 before the products have looked for tile n, but not
   // with tile n + 2, whose scores are issued behind the values of tile n.
-  uint64_t p_full[C::NWG][2];
-  uint64_t o_done[C::NWG][2];  // O^T += V^T P^T complete, tiles in turn
+  uint64_t p_full[2];
+  uint64_t o_done[2];        // O^T += V^T P^T complete, tiles in turn
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -388,13 +416,12 @@ struct __align__(16) Shared {
 struct Row {
   int b, h, i;
   __device__ __forceinline__ Row(const Args& a, int seq, int hk, int j) {
-    const int n = a.seqlen_q * a.group;
     b = seq;
     if (a.prefix_mode) {
-      b = j / n;
-      j -= b * n;
+      b = a.by_seq_rows.div(j);
+      j -= b * a.by_seq_rows.d;
     }
-    i = j / a.group;
+    i = a.by_group.div(j);
     h = hk * a.group + j - i * a.group;
   }
 };
@@ -439,12 +466,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     if (lane < 2) {
       ptx::mbar_init(&sh.q_full[lane], C::kQWarps);
       ptx::mbar_init(&sh.q_free[lane], C::NWG * 4);
-    }
-    if (lane < C::NWG) {
-      ptx::mbar_init(&sh.p_full[lane][0], 4);
-      ptx::mbar_init(&sh.p_full[lane][1], 4);
-      ptx::mbar_init(&sh.o_done[lane][0], 1);
-      ptx::mbar_init(&sh.o_done[lane][1], 1);
+      ptx::mbar_init(&sh.p_full[lane], C::NWG * 4);
+      ptx::mbar_init(&sh.o_done[lane], 1);
     }
     if (lane == 0) {
       ptx::mbar_init(&sh.s_full, 1);
@@ -502,50 +525,56 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       }
       const int item = (u0 - at) / walk.nt;
       walk.t = u0 - at - item * walk.nt;
-      walk.hk = item / a.row_tiles;
+      walk.hk = a.by_row_tiles.div(item);
       walk.rt = item - walk.hk * a.row_tiles;
     }
   }
 
   // Sequences without a key among these items have no tile and no block of
   // their own: their rows (items) are filled in by block b mod G.
-  if (!a.prefix_mode) {
+  auto fill_empty = [&](int first, int step) {
+    if (a.prefix_mode) return;
     for (int b = cta; b < a.c.batch; b += G) {
       const int len = seq_len(a, b);
       if (len < 0 || tiles_of(a, len) > 0) continue;
       if (a.own_rows) {
         const int n = a.heads * a.seqlen_q;
-        for (int j = threadIdx.x; j < n * (D / 8); j += C::kThreads) {
+        for (int j = first; j < n * (D / 8); j += step) {
           const int row = j / (D / 8), h = row / a.seqlen_q, i = row - h * a.seqlen_q;
           reinterpret_cast<uint4*>(a.o + 2 * (b * a.o_sb + h * a.o_sh + i * a.o_ss))[j % (D / 8)] =
               make_uint4(0, 0, 0, 0);
           if (a.lse && j % (D / 8) == 0) a.lse[(long long)b * n + row] = -INFINITY;
         }
       } else {
-        for (int j = threadIdx.x; j < per; j += C::kThreads)
+        for (int j = first; j < per; j += step)
           a.item[(long long)b * per + j] = make_int4(0, 0, 0, kItemEmpty);
       }
     }
-  }
+  };
   if (a.own_rows && threadIdx.x == 0) a.seg[cta] = make_int4(-1, 0, 0, 0);
-  ptx::tc_fence_before();
-  __syncthreads();
-  ptx::tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  // Barriers and TMEM are there for all. Every role comes here when it has
+  // asked for its first data.
+  auto block_sync = [&]() {
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+  };
   if (u0 == u1) {
-    if (warp == C::kMmaWarp) ptx::tmem_dealloc(tmem, C::kTmemCols);
+    block_sync();
+    if (warp == C::kMmaWarp) ptx::tmem_dealloc(sh.tmem, C::kTmemCols);
+    fill_empty(threadIdx.x, C::kThreads);
     if (a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  // Ring of K and V tiles | P of each warpgroup | Q of two items, each of all
-  // warpgroups.
+  // Ring of K and V tiles | P | Q of two items.
   uint8_t* const p_tiles = smem + NS * C::kSlotBytes;
-  uint8_t* const q_tiles = p_tiles + C::NWG * C::kPBufs * C::kPBytes;
+  uint8_t* const q_tiles = p_tiles + C::kPBufs * C::kPBytes;
   const Waiter wait{&sh.abort, a.c.status, a.timeout};
   Seg s;
+  bool more = walk.next(a, s);
 
   if (warp >= C::kMmaWarp) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsHelp));
@@ -566,13 +595,14 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     }
     int n = 0, issued = 0;
     bool ok = true;
-    while (ok && walk.next(a, s)) {
+    for (bool first = true; ok && more; more = walk.next(a, s), first = false) {
       const int* table = a.c.table + (a.prefix_mode ? 0 : s.b) * a.c.table_stride;
       auto entry = [&](int t) {
         const int key = a.key_base + t * kTileKeys + lane * a.box;
         return lane < pieces && key < s.len ? __ldg(table + page_of(a, key)) : 0;
       };
       int page = entry(s.t0);
+      if (first) block_sync();
       for (int t = s.t0; t < s.t1; ++t, ++n) {
         const int next = t + 1 < s.t1 ? entry(t + 1) : 0;
         const int key0 = a.key_base + t * kTileKeys, key = key0 + lane * a.box;
@@ -635,12 +665,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     // the two warps takes every other batch of rows.
     constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row; rows at a time
     constexpr int kHalf = C::kRows / C::kQWarps / kPer;
-    constexpr int kMost = C::NWG > 1 ? 8 : 4;           // loads in flight
+    constexpr int kMost = 4;                            // loads in flight
     constexpr int kBatch = kHalf < kMost ? kHalf : kMost;
     static_assert(C::kRows % (kPer * kBatch * C::kQWarps) == 0, "whole batches");
     const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
     const int me = warp - C::kQWarp;
-    for (int k = 0; walk.next(a, s); ++k) {
+    block_sync();
+    for (int k = 0; more; more = walk.next(a, s), ++k) {
       const int buf = k & 1;
       if (k >= 2 && !wait.warp(&sh.q_free[buf], ((k >> 1) - 1) & 1)) break;
       auto& rw = sh.rows[buf];
@@ -731,13 +762,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       if (lane == 0) ptx::mbar_arrive(&sh.q_full[buf]);
     }
   } else if (warp == C::kMmaWarp) {
+    block_sync();
     if (lane == 0) {
       // ------------------------------------------------------------ MMA issuer
+      const uint32_t tmem = sh.tmem;
       const uint32_t ring = ptx::smem_u32(smem), pb = ptx::smem_u32(p_tiles),
                      qb = ptx::smem_u32(q_tiles);
-      // One product for the scores of all warpgroups, one for each one's values.
+      // One product for all warpgroups: an instruction costs the issuing thread
+      // some 100 clocks whatever its N (one product of values per warpgroup
+      // made this thread the slowest of all: 5000 clocks a tile of 64 rows).
       constexpr uint32_t idesc_s = ptx::idesc_e4m3_f32(128, C::NWG * C::kN);
-      constexpr uint32_t idesc_o = idesc_tt(128, C::kN);
+      constexpr uint32_t idesc_o = idesc_tt(128, C::NWG * C::kN);
       bool ok = true;
       auto scores = [&](int n, int k, bool first) {  // S^T of tile n, in item k
         const int i = 2 * n, st = i % NS;
@@ -757,26 +792,23 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       auto values = [&](int n, bool first) {  // O^T += V^T P^T of tile n
         const int i = 2 * n + 1, st = i % NS;
         ok = wait(&sh.kv_full[st], (i / NS) & 1);
+        ok = ok && wait(&sh.p_full[n & 1], (n >> 1) & 1);
+        if (!ok) return;
+        ptx::tc_fence_after();
+        const uint32_t p = pb + n % C::kPBufs * C::kPBytes;
 #pragma unroll
-        for (int w = 0; w < C::NWG; ++w) {
-          ok = ok && wait(&sh.p_full[w][n & 1], (n >> 1) & 1);
-          if (!ok) return;
-          ptx::tc_fence_after();
-          const uint32_t p = pb + (w * C::kPBufs + n % C::kPBufs) * C::kPBytes;
-#pragma unroll
-          for (int kk = 0; kk < kTileKeys / 32; ++kk)
-            ptx::umma_f8(tmem + (C::NWG + w) * C::kN, desc_v<D>(ring + st * C::kSlotBytes + kk * 32 * D),
-                         ptx::smem_desc_mnmajor(p + kk * 32 * C::kPitch, C::kPitch), idesc_o,
-                         first && kk == 0 ? 0u : 1u);
-          ptx::umma_commit(&sh.o_done[w][n & 1]);
-        }
+        for (int kk = 0; kk < kTileKeys / 32; ++kk)
+          ptx::umma_f8(tmem + C::NWG * C::kN, desc_v<D>(ring + st * C::kSlotBytes + kk * 32 * D),
+                       desc_p<C::kPitch>(p + kk * 32 * C::kPitch), idesc_o,
+                       first && kk == 0 ? 0u : 1u);
+        ptx::umma_commit(&sh.o_done[n & 1]);
         ptx::umma_commit(&sh.kv_empty[st]);
       };
       // The scores of the next tile, be it the next item's first, are issued
       // before this tile's values: they are ready when its softmax is done.
       int n = 0, k = 0;
-      if (walk.next(a, s)) scores(0, 0, true);
-      for (bool more = true; ok && more; ++k) {
+      scores(0, 0, true);
+      for (; ok && more; ++k) {
         const int count = s.t1 - s.t0;
         for (int j = 0; ok && j < count; ++j, ++n) {
           if (j + 1 < count) {
@@ -795,6 +827,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     // --------------------------------------------------------------- softmax
+    block_sync();
+    fill_empty(threadIdx.x, C::NWG * 128);  // (nothing to do yet)
+    const uint32_t tmem = sh.tmem;
     const int w = warp / 4, wq = warp % 4, tid = threadIdx.x % 128;
     auto& g = sh.g[w];
     bool ok = true;
@@ -815,7 +850,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     // A warp whose wait gave up goes on to the next barrier, and all four
     // leave there together.
     bool left = false;
-    for (; walk.next(a, s); ++k) {
+    for (; more; more = walk.next(a, s), ++k) {
       const auto& rw = sh.rows[k & 1];
       ok = ok && wait.warp(&sh.q_full[k & 1], (k >> 1) & 1);
       const int all_see = min(rw.all_see[0], rw.all_see[1]);
@@ -902,7 +937,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         // P's buffer is free: the product that read it two tiles ago was
         // issued before these scores, whose completion covers it. With one
         // buffer the product of the tile before has to be waited for.
-        if (C::kPBufs == 1 && n > 0) ok = ok && wait.warp(&sh.o_done[w][(n - 1) & 1], ((n - 1) >> 1) & 1);
+        if (C::kPBufs == 1 && n > 0) ok = ok && wait.warp(&sh.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
         if (rise) {
           float top = -INFINITY;
 #pragma unroll
@@ -946,7 +981,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
           if (t > s.t0) {
             // The sums so far, rescaled; O when the tile before is in it.
             const uint32_t rose = __ballot_sync(0xffffffffu, f_lane != 1.f);
-            ok = ok && wait.warp(&sh.o_done[w][(n - 1) & 1], ((n - 1) >> 1) & 1);
+            ok = ok && wait.warp(&sh.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
             ptx::tc_fence_after();
 #pragma unroll
             for (int c = 0; c < RW; c += 8) {
@@ -976,7 +1011,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         // p, its sum, and the key's row of P: the terms side by side. A key
         // that some rows do not see may have a NaN factor: their product with
         // it is then not formed (kPick).
-        uint8_t* const p_tile = p_tiles + (w * C::kPBufs + n % C::kPBufs) * C::kPBytes;
+        uint8_t* const p_tile = p_tiles + n % C::kPBufs * C::kPBytes;
         auto emit = [&](auto pick) {
           constexpr bool kPick = decltype(pick)::value;
           const uint64_t vf2 = ptx::pack2(vf, vf);
@@ -999,7 +1034,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
               terms8<NT>(y[0], y[1], y[2], y[3], t8);
 #pragma unroll
               for (int q = 0; q < NT; ++q)
-                *reinterpret_cast<uint2*>(p_tile + swz<C::kPitch>(tid, q * RW + c)) = t8[q];
+              {
+                const int col = w * C::kN + q * RW + c;
+                *reinterpret_cast<uint2*>(p_tile + col / C::kPitch * (kTileKeys * C::kPitch) +
+                                          swz<C::kPitch>(tid, col % C::kPitch)) = t8[q];
+              }
             }
           }
         };
@@ -1021,7 +1060,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&sh.p_full[w][n & 1]);
+        if (lane == 0) ptx::mbar_arrive(&sh.p_full[n & 1]);
       }
       if (left) break;
 
@@ -1034,7 +1073,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         constexpr int kEach = 32 / RW;  // lanes that hold the same row's sum
         if (lane % kEach == 0) reinterpret_cast<float*>(&g.sum[lane / kEach])[wq] = v;
       }
-      ok = ok && wait.warp(&sh.o_done[w][(n - 1) & 1], ((n - 1) >> 1) & 1);
+      ok = ok && wait.warp(&sh.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
       ptx::tc_fence_after();
       if (any_of(!ok)) break;
       const bool begins = s.t0 == 0, whole = begins && s.t1 == s.nt;
@@ -1109,7 +1148,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
   __syncthreads();
   if (warp == C::kMmaWarp) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, C::kTmemCols);
+    ptx::tmem_dealloc(sh.tmem, C::kTmemCols);
   }
   // A launch that overlaps the one before it ends after it: whoever waits for
   // this one has both.
@@ -1346,10 +1385,10 @@ struct Shape {
 Shape shape_for(int64_t rows) {
   if (rows <= 8) return {8, 1};
   if (rows <= 16) return {16, 1};
-  if (rows <= 32) return {32, 1};
-  return {32, 2};
+  if (rows <= 32) return {16, 2};
+  return {16, 4};
 }
-int ctas_per_sm(int64_t d, const Shape& s) { return s.nwg > 1 ? 1 : (d == 64 && s.rw == 8 ? 3 : 2); }
+int ctas_per_sm(int64_t d, const Shape& s) { return s.nwg > 2 ? 1 : (d == 64 && s.rw == 8 ? 3 : 2); }
 
 constexpr int kSmCount = 148;
 
@@ -1427,6 +1466,7 @@ int run_set(const fa8_decode_params* p, Args a, const Layout& l, char* ws, int d
   constexpr int NT = kBf16 ? 2 : 3;
   const fa8_kv_cache& c = p->cache;
   a.row_tiles = (int)l.row_tiles;
+  a.by_row_tiles = Divisor::of(a.row_tiles);
   a.part_o = reinterpret_cast<float*>(ws + l.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
   a.seg = reinterpret_cast<int4*>(ws + l.seg);
@@ -1438,8 +1478,8 @@ int run_set(const fa8_decode_params* p, Args a, const Layout& l, char* ws, int d
   if (!st) st = make_map(&tv, c, c.v, c.v_stride_p, c.v_stride_h, c.v_stride_s, a.box, ws);
   if (st) return st;
   const int grid = (int)l.grid;
-  if (l.shape.nwg == 2) return launch_set<Cfg<D, NT, 32, 2>, kBf16>(a, tk, tv, grid, dev, stream);
-  if (l.shape.rw == 32) return launch_set<Cfg<D, NT, 32, 1>, kBf16>(a, tk, tv, grid, dev, stream);
+  if (l.shape.nwg == 4) return launch_set<Cfg<D, NT, 16, 4>, kBf16>(a, tk, tv, grid, dev, stream);
+  if (l.shape.nwg == 2) return launch_set<Cfg<D, NT, 16, 2>, kBf16>(a, tk, tv, grid, dev, stream);
   if (l.shape.rw == 16) return launch_set<Cfg<D, NT, 16, 1>, kBf16>(a, tk, tv, grid, dev, stream);
   return launch_set<Cfg<D, NT, 8, 1>, kBf16>(a, tk, tv, grid, dev, stream);
 }
@@ -1549,8 +1589,9 @@ int fa8_decode(const fa8_decode_params* p, void* workspace, int64_t workspace_by
   a.prefix_len = (int)p->prefix_len;
   const int page = (int)p->cache.page_size;
   a.box = std::min(page, kTileKeys);
-  while ((1 << a.page_shift) < page) ++a.page_shift;
-  a.page_mul = (uint32_t)((((1ull << a.page_shift) - page) << 32) / page + 1);
+  a.by_page = Divisor::of(page);
+  a.by_group = Divisor::of(a.group);
+  a.by_seq_rows = Divisor::of(a.group * a.seqlen_q);
   a.q_sb = p->q_stride_b;
   a.q_sh = p->q_stride_h;
   a.q_ss = p->q_stride_s;
