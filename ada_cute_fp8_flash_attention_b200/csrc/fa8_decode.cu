@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     // the two warps takes every other batch of rows.
     constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row; rows at a time
     constexpr int kHalf = C::kRows / C::kQWarps / kPer;
-    constexpr int kMost = 4;                            // loads in flight
+    constexpr int kMost = C::kRegsHelp < 80 ? 2 : 4;     // loads in flight
     constexpr int kBatch = kHalf < kMost ? kHalf : kMost;
     static_assert(C::kRows % (kPer * kBatch * C::kQWarps) == 0, "whole batches");
     const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
@@ -718,42 +718,59 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       if (lane == 0) rw.all_see[me] = see;
 #pragma unroll 1
       for (int r0 = me * kPer * kBatch; r0 < filled; r0 += C::kQWarps * kPer * kBatch) {
+        // Stage by stage over the batch: a warp by itself is as fast as its
+        // chains are side by side.
+        uint32_t top[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const uint32_t m = __vmaxu2(__vmaxu2(xs[u].x & 0x7fff7fffu, xs[u].y & 0x7fff7fffu),
+                                      __vmaxu2(xs[u].z & 0x7fff7fffu, xs[u].w & 0x7fff7fffu));
+          top[u] = max(m & 0xffffu, m >> 16);
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o; o >>= 1) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u)
+            top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+        }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
           const int r = r0 + u * kPer + lane / kLanes;
-          const uint4 x = xs[u];
-          uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-          m = max(m & 0xffffu, m >> 16);
-#pragma unroll
-          for (int o = kLanes / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const uint32_t m = top[u];
           const bool fine = m < (kBf16 ? 0x7f80u : 0x7c00u);
           const uint32_t bits =
               kBf16 ? m << 16
                     : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
           // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
           const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
+          if (cl == 0)
+            rw.mul[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
+                             : __int_as_float(0x7fc00000);
           const float f = fine ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
-          uint32_t hx[4];
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const uint32_t word = q4 == 0 ? x.x : q4 == 1 ? x.y : q4 == 2 ? x.z : x.w;
+          auto scale2 = [&](uint32_t word) -> uint32_t {
             float2 v;
             if (kBf16)
               v = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
             else
               v = __half22float2(*reinterpret_cast<const __half2*>(&word));
-            hx[q4] = fine ? h2(v.x * f, v.y * f) : 0u;
-          }
-          uint2 t8[NT];
-          terms8<NT>(hx[0], hx[1], hx[2], hx[3], t8);
-          uint8_t* const q_tile = q_tiles + (buf * C::NWG + r / RW) * C::kQBytes;
+            return fine ? h2(v.x * f, v.y * f) : 0u;
+          };
+          xs[u] = make_uint4(scale2(xs[u].x), scale2(xs[u].y), scale2(xs[u].z), scale2(xs[u].w));
+        }
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-            *reinterpret_cast<uint2*>(q_tile + swz<D>(t * RW + r % RW, cl * 8)) = t8[t];
-          if (cl == 0)
-            rw.mul[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
-                             : __int_as_float(0x7fc00000);
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int r = r0 + u * kPer + lane / kLanes;
+            const uint16_t e0 = e4m3x2_of_h2(xs[u].x), e1 = e4m3x2_of_h2(xs[u].y),
+                           e2 = e4m3x2_of_h2(xs[u].z), e3 = e4m3x2_of_h2(xs[u].w);
+            *reinterpret_cast<uint2*>(q_tiles + (buf * C::NWG + r / RW) * C::kQBytes +
+                                      swz<D>(t * RW + r % RW, cl * 8)) =
+                make_uint2((uint32_t)e0 | ((uint32_t)e1 << 16), (uint32_t)e2 | ((uint32_t)e3 << 16));
+            if (t + 1 < NT)
+              xs[u] = make_uint4(rest(xs[u].x, e0), rest(xs[u].y, e1), rest(xs[u].z, e2),
+                                 rest(xs[u].w, e3));
+          }
         }
         ask(r0 + C::kQWarps * kPer * kBatch);
       }
@@ -1073,8 +1090,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         constexpr int kEach = 32 / RW;  // lanes that hold the same row's sum
         if (lane % kEach == 0) reinterpret_cast<float*>(&g.sum[lane / kEach])[wq] = v;
       }
-      ok = ok && wait.warp(&sh.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
-      ptx::tc_fence_after();
       if (any_of(!ok)) break;
       const bool begins = s.t0 == 0, whole = begins && s.t1 == s.nt;
       const int part = 2 * cta + (k > 0 ? 1 : 0);
@@ -1104,6 +1119,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
           a.item[(long long)s.b * per + s.hk * a.row_tiles + s.rt] =
               make_int4(cta, last, part, whole ? kItemFull : kItemParts);
       }
+      // (Should this wait give up, the next barrier ends the block.)
+      ok = ok && wait.warp(&sh.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+      ptx::tc_fence_after();
       // O^T: a thread has one d of every row; with D = 64 the upper half of the
       // lanes repeats the lower and takes the odd rows.
       const int d = tid % D;

@@ -444,6 +444,7 @@ int64_t stride_or(const torch::Tensor& t, int64_t d, int64_t dflt) {
 }
 
 torch::Tensor device_i32(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
+  if (t.scalar_type() == at::kInt && t.device() == like.device()) return t;
   TORCH_CHECK(t.device().is_cpu() || t.device() == like.device(), name,
               " must be on the cache's device (or on the host)");
   TORCH_CHECK(at::isIntegralType(t.scalar_type(), false), name, " must hold integers");
