@@ -63,6 +63,7 @@ namespace fa8 {
 namespace dec {
 
 constexpr int kTileKeys = 128;
+constexpr int kMostItemCost = 8;
 constexpr float kRise = 5.f;           // log2 of the rise of a maximum that is let be
 constexpr float kPScale = 8.f;         // 8 p 2^e <= 2^(3 + kRise) < 448
 constexpr float kTerm = 16.f;          // weight of a term over the next
@@ -84,6 +85,11 @@ struct Cfg {
   static constexpr int kQWarps = 2;
   static constexpr int kN = (NT * RW + 15) / 16 * 16;  // columns of the products
   static constexpr int kStep = NWG == 1 ? RW : 8;     // rows read from TMEM at a time
+  // What an item costs a block beside its tiles, in tiles: its rows, its first
+  // maximum, its result. Without it the blocks with most items were the last
+  // by far (37000 clocks with one item, 61000 with four, the same tiles).
+  static constexpr int kItemCost = NWG == 1 ? 2 : 4;
+  static_assert(kItemCost <= kMostItemCost, "the host's bound of a share");
   // P of all warpgroups side by side: bytes of a key's row, in atoms of up to
   // 128 (three terms of 64 rows take one and a half).
   static constexpr int kPCols = NWG * kN;
@@ -315,51 +321,54 @@ __device__ __forceinline__ int tiles_of(const Args& a, int len) {
 // A run of key tiles t0..t1-1 of one item (sequence b, K/V head, row tile).
 struct Seg {
   int b, hk, rt, t0, t1, nt, len;
-  int unit;  // number of tile t0 among all
+  int end;  // number of the item's last unit among all
 };
 
-// Walks a block's share of the tiles; every role of the block walks the same.
+// Walks a block's share; every role of the block walks the same. Work is
+// numbered in units: an item has `cost` for itself and then one per tile.
 struct Walk {
-  int b, hk, rt, t, nt, len;
+  int b, hk, rt, off, nt, len;  // off: units of the item that lie behind
   int unit, left;
   __device__ __forceinline__ void enter(const Args& a) {
     len = seq_len(a, b);
     nt = tiles_of(a, len);
   }
-  __device__ __forceinline__ bool next(const Args& a, Seg& s) {
-    if (left == 0) return false;
-    while (nt == 0) {
-      ++b;
-      enter(a);
-    }
-    s.b = b;
-    s.hk = hk;
-    s.rt = rt;
-    s.t0 = t;
-    s.nt = nt;
-    s.len = len;
-    const int n = min(nt - t, left);
-    s.t1 = t + n;
-    s.unit = unit;
-    left -= n;
-    unit += n;
-    t = s.t1;
-    if (t == nt) {
-      t = 0;
-      if (++rt == a.row_tiles) {
-        rt = 0;
-        if (++hk == a.c.heads_kv) {
-          hk = 0;
-          ++b;
-          if (left > 0) enter(a);
+  __device__ __forceinline__ bool next(const Args& a, int cost, Seg& s) {
+    while (left > 0) {
+      while (nt == 0) {
+        ++b;
+        enter(a);
+      }
+      s.b = b;
+      s.hk = hk;
+      s.rt = rt;
+      s.nt = nt;
+      s.len = len;
+      s.end = unit - off + cost + nt - 1;
+      s.t0 = max(0, off - cost);
+      const int take = min(cost + nt - off, left);
+      off += take;
+      unit += take;
+      left -= take;
+      s.t1 = max(0, off - cost);
+      if (off == cost + nt) {
+        off = 0;
+        if (++rt == a.row_tiles) {
+          rt = 0;
+          if (++hk == a.c.heads_kv) {
+            hk = 0;
+            ++b;
+            if (left > 0) enter(a);
+          }
         }
       }
+      if (s.t1 > s.t0) return true;
     }
-    return true;
+    return false;
   }
 };
 
-// Shares of `total` tiles over `n` blocks: the first total % n have one more.
+// Shares of `total` units over `n` blocks: the first total % n have one more.
 struct Shares {
   int size, more;
   __device__ __forceinline__ Shares(int total, int n) : size(total / n), more(total - size * n) {}
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
   }
 
   // ------------------------------------------------- this block's share
-  // Every warp finds it for itself: lane i counts the tiles of a run of
+  // Every warp finds it for itself: lane i counts the units of a run of
   // sequences, a scan says how many come before. (The host has checked that
   // they number less than 2^31.)
   const int nseq = a.prefix_mode ? 1 : a.c.batch;
@@ -493,7 +502,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     const int len = seq_len(a, b);
     if (len < 0 && cta == 0 && warp == 0 && a.c.status)
       atomicOr(a.c.status, FA8_DEVERR_VARLEN_RANGE);
-    mine += per * tiles_of(a, len);
+    const int nt = tiles_of(a, len);
+    mine += nt > 0 ? per * (C::kItemCost + nt) : 0;
   }
   if (warp == C::kMmaWarp) {
     ptx::tmem_alloc(&sh.tmem, C::kTmemCols);
@@ -506,7 +516,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     if (lane >= o) upto += v;
   }
   const int total = __shfl_sync(0xffffffffu, upto, 31);
-  const int active = min(G, total);  // blocks with work: a tile at least
+  const int active = min(G, total);  // blocks with a share
   const Shares shares(total, max(active, 1));
   const int u0 = cta < active ? shares.begin(cta) : 0;
   const int u1 = cta < active ? shares.begin(cta + 1) : 0;
@@ -515,16 +525,18 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
   walk.unit = u0;
   {
     const uint32_t here = __ballot_sync(0xffffffffu, u0 >= upto - mine && u0 < upto);
-    const int src = __ffs(here) - 1;  // the lane in whose sequences tile u0 is
+    const int src = __ffs(here) - 1;  // the lane in whose sequences unit u0 is
     if (u0 < u1) {
       int at = __shfl_sync(0xffffffffu, upto - mine, src);
       for (walk.b = __shfl_sync(0xffffffffu, s0, src);; ++walk.b) {
         walk.enter(a);
-        if (u0 < at + per * walk.nt) break;
-        at += per * walk.nt;
+        if (walk.nt == 0) continue;
+        const int n = per * (C::kItemCost + walk.nt);
+        if (u0 < at + n) break;
+        at += n;
       }
-      const int item = (u0 - at) / walk.nt;
-      walk.t = u0 - at - item * walk.nt;
+      const int each = C::kItemCost + walk.nt, item = (u0 - at) / each;
+      walk.off = u0 - at - item * each;
       walk.hk = a.by_row_tiles.div(item);
       walk.rt = item - walk.hk * a.row_tiles;
     }
@@ -559,7 +571,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     __syncthreads();
     ptx::tc_fence_after();
   };
-  if (u0 == u1) {
+  Seg s;
+  bool more = walk.next(a, C::kItemCost, s);
+  if (!more) {  // no share, or one that ends before its item's first tile
     block_sync();
     if (warp == C::kMmaWarp) ptx::tmem_dealloc(sh.tmem, C::kTmemCols);
     fill_empty(threadIdx.x, C::kThreads);
@@ -573,9 +587,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
   uint8_t* const p_tiles = smem + NS * C::kSlotBytes;
   uint8_t* const q_tiles = p_tiles + C::kPBufs * C::kPBytes;
   const Waiter wait{&sh.abort, a.c.status, a.timeout};
-  Seg s;
-  bool more = walk.next(a, s);
-
   if (warp >= C::kMmaWarp) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsHelp));
   if (warp == C::kLoadWarp) {
@@ -595,7 +606,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     }
     int n = 0, issued = 0;
     bool ok = true;
-    for (bool first = true; ok && more; more = walk.next(a, s), first = false) {
+    for (bool first = true; ok && more; more = walk.next(a, C::kItemCost, s), first = false) {
       const int* table = a.c.table + (a.prefix_mode ? 0 : s.b) * a.c.table_stride;
       auto entry = [&](int t) {
         const int key = a.key_base + t * kTileKeys + lane * a.box;
@@ -671,7 +682,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
     const int me = warp - C::kQWarp;
     block_sync();
-    for (int k = 0; more; more = walk.next(a, s), ++k) {
+    for (int k = 0; more; more = walk.next(a, C::kItemCost, s), ++k) {
       const int buf = k & 1;
       if (k >= 2 && !wait.warp(&sh.q_free[buf], ((k >> 1) - 1) & 1)) break;
       auto& rw = sh.rows[buf];
@@ -831,7 +842,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
           if (j + 1 < count) {
             scores(n + 1, k, false);
           } else {
-            more = walk.next(a, s);
+            more = walk.next(a, C::kItemCost, s);
             if (more) scores(n + 1, k + 1, true);
           }
           if (ok) values(n, j == 0);
@@ -867,7 +878,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     // A warp whose wait gave up goes on to the next barrier, and all four
     // leave there together.
     bool left = false;
-    for (; more; more = walk.next(a, s), ++k) {
+    for (; more; more = walk.next(a, C::kItemCost, s), ++k) {
       const auto& rw = sh.rows[k & 1];
       ok = ok && wait.warp(&sh.q_full[k & 1], (k >> 1) & 1);
       const int all_see = min(rw.all_see[0], rw.all_see[1]);
@@ -1112,7 +1123,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       }
       if (w == 0 && tid == 0 && begins && !(a.own_rows && whole)) {
         // Says where the item's parts are: from this block to its last tile's.
-        const int last = whole ? cta : shares.block_of(s.unit + s.nt - 1);
+        const int last = whole ? cta : shares.block_of(s.end);
         if (a.own_rows)
           a.seg[cta] = make_int4(last, s.b, s.hk * a.row_tiles + s.rt, part);
         else
@@ -1332,9 +1343,10 @@ int check(const fa8_decode_params* p, bool* empty) {
     return fa8_note_error(FA8_ERR_UNSUPPORTED, "fa8_decode: too many query rows");
   if (p->prefix_len > p->cache.max_pages * p->cache.page_size)
     return fa8_note_error(FA8_ERR_INVALID_ARG, "fa8_decode: prefix_len does not fit the page table");
-  // Key tiles of all items number less than 2^31, whatever the lengths are.
+  // The units of work number less than 2^31, whatever the lengths are.
   const int64_t group = p->heads / p->cache.heads_kv;
-  const int64_t tiles = (p->cache.max_pages * p->cache.page_size + 2 * kTileKeys - 1) / kTileKeys;
+  const int64_t tiles =
+      (p->cache.max_pages * p->cache.page_size + 2 * kTileKeys - 1) / kTileKeys + kMostItemCost;
   for (int64_t rows : {p->seqlen_q * group, p->seqlen_q * group * p->cache.batch}) {
     const int64_t seqs = rows == p->seqlen_q * group ? p->cache.batch : 1;
     if (seqs * p->cache.heads_kv * ((rows + 7) / 8) > (1ll << 31) / tiles - 1)
