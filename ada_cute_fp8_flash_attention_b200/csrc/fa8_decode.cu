@@ -74,6 +74,12 @@ constexpr int kWaitHintNs = 20000;
 // behind it.
 enum { kItemEmpty = 0, kItemFull = 1, kItemParts = 2 };
 
+// Blocks an SM holds: what four warpgroups leave of TMEM, else what registers
+// and the ring do (D = 64 has half the tile, and needs more of them in flight).
+constexpr int resident(int d, int rw, int nwg) {
+  return nwg > 2 ? 1 : (d == 64 && rw == 8 ? 3 : 2);
+}
+
 // D: head dimension. NT: e4m3 terms of Q and P (2 bf16, 3 fp16). RW: query
 // rows of a softmax warpgroup. NWG: warpgroups, each with its own rows.
 template <int D_, int NT_, int RW_, int NWG_>
@@ -100,8 +106,12 @@ struct Cfg {
   static constexpr int kPBytes = kTileKeys * kPitch * kPAtoms;
   static constexpr uint32_t kTmemUsed = 2u * kN * NWG;
   static constexpr uint32_t kTmemCols =
-      kTmemUsed <= 32 ? 32 : kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
-  static constexpr int kCtas = NWG > 2 ? 1 : (D == 64 && RW == 8 ? 3 : 2);  // per SM
+      kTmemUsed <= 32    ? 32
+      : kTmemUsed <= 64  ? 64
+      : kTmemUsed <= 128 ? 128
+      : kTmemUsed <= 256 ? 256
+                         : 512;
+  static constexpr int kCtas = resident(D, RW, NWG);
   // 227 KB a block, 228 KB an SM of which each block takes 1 KB and its
   // static variables; 1 KB to align.
   static constexpr int kStatic = 2688 + 80 * kRows;
@@ -156,7 +166,7 @@ struct Args {
   int prefix_len;
   int row_tiles;     // tiles of query rows per (sequence, K/V head)
   int box;           // keys of a TMA box: min(page_size, 128)
-  Divisor by_page, by_group, by_seq_rows, by_row_tiles;  // page_size, group, group * seqlen_q, row_tiles
+  Divisor by_page, by_group, by_seq_rows, by_row_tiles;  // (by_seq_rows: group * seqlen_q)
   int own_rows;      // results go to o (1), or to full_* and item (0)
   int early;         // this launch may overlap the one before it
   float scale_log2;
@@ -302,9 +312,11 @@ struct Waiter {
     return __all_sync(0xffffffffu, (*this)(bar, parity));
   }
 };
-__device__ __forceinline__ void wait_quietly(uint64_t* bar, uint32_t parity, long long limit) {
+// For what is in flight when a block ends: bounded too, but not by the caller,
+// whose limit may be shorter than a copy takes.
+__device__ __forceinline__ void wait_quietly(uint64_t* bar, uint32_t parity) {
   const long long t0 = clock64();
-  while (!ptx::mbar_try_wait(bar, parity) && clock64() - t0 < limit) {
+  while (!ptx::mbar_try_wait(bar, parity) && clock64() - t0 < kTimeout) {
   }
 }
 
@@ -417,7 +429,8 @@ struct __align__(16) Shared {
     float4 top[C::RW];       // and maxima of a tile
   } g[C::NWG];
   static_assert(sizeof(Rows) % 16 == 0 && sizeof(Group) % 16 == 0, "read four at a time");
-  static_assert(C::kSlots / 2 + 2 <= kExpTiles, "a tile's exponents are read before their place is used again");
+  static_assert(C::kSlots / 2 + 2 <= kExpTiles,
+                "a tile's exponents are read before their place is used again");
 };
 
 // Row j of item rows (K/V head hk; sequence b unless the items are the
@@ -588,270 +601,270 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
   uint8_t* const q_tiles = p_tiles + C::kPBufs * C::kPBytes;
   const Waiter wait{&sh.abort, a.c.status, a.timeout};
   if (warp >= C::kMmaWarp) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsHelp));
-  if (warp == C::kLoadWarp) {
-    // ------------------------------------------------------------ TMA producer
-    // Lane l brings piece l (box keys of one page) of a K and of a V tile.
-    // Ring item 2n is K of the block's tile n, 2n + 1 its V. Lanes 0-15 bring
-    // the tile's exponent bytes, 16 keys of K or V each.
-    const int pieces = kTileKeys / a.box;
-    const uint64_t policy = a.row_tiles > 1 ? ptx::policy_evict_last() : ptx::policy_evict_first();
-    const bool is_v = lane >= 8;
-    const int e_key = (lane & 7) * 16, e_piece = e_key / a.box;
-    const uint8_t* const exps = is_v ? a.c.v_exp : a.c.k_exp;
-    const long long e_sp = is_v ? a.c.ve_sp : a.c.ke_sp, e_sh = is_v ? a.c.ve_sh : a.c.ke_sh;
-    if (lane == 0) {
-      ptx::tma_prefetch_desc(&tm_k);
-      ptx::tma_prefetch_desc(&tm_v);
-    }
-    int n = 0, issued = 0;
-    bool ok = true;
-    for (bool first = true; ok && more; more = walk.next(a, C::kItemCost, s), first = false) {
-      const int* table = a.c.table + (a.prefix_mode ? 0 : s.b) * a.c.table_stride;
-      auto entry = [&](int t) {
-        const int key = a.key_base + t * kTileKeys + lane * a.box;
-        return lane < pieces && key < s.len ? __ldg(table + page_of(a, key)) : 0;
-      };
-      int page = entry(s.t0);
-      if (first) block_sync();
-      for (int t = s.t0; t < s.t1; ++t, ++n) {
-        const int next = t + 1 < s.t1 ? entry(t + 1) : 0;
-        const int key0 = a.key_base + t * kTileKeys, key = key0 + lane * a.box;
-        const bool have = lane < pieces && key < s.len;
-        // A page outside the cache: coordinates that read as zeros, exponents
-        // that say NaN.
-        const bool outside = page < 0 || page >= a.c.num_pages;
-        if (have && outside && a.c.status) atomicOr(a.c.status, FA8_DEVERR_PAGE_RANGE);
-        const int coord = outside ? 0x7fffffff : page;
-        const int slot = key - page_of(a, key) * a.c.page_size;
-        const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, have)) * a.box * D;
-        const int e_coord = __shfl_sync(0xffffffffu, coord, e_piece);
-        const int e_slot = __shfl_sync(0xffffffffu, slot, e_piece) + e_key - e_piece * a.box;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsHelp));
+    if (warp == C::kLoadWarp) {
+      // ------------------------------------------------------------ TMA producer
+      // Lane l brings piece l (box keys of one page) of a K and of a V tile.
+      // Ring item 2n is K of the block's tile n, 2n + 1 its V. Lanes 0-15 bring
+      // the tile's exponent bytes, 16 keys of K or V each.
+      const int pieces = kTileKeys / a.box;
+      const uint64_t policy = a.row_tiles > 1 ? ptx::policy_evict_last() : ptx::policy_evict_first();
+      const bool is_v = lane >= 8;
+      const int e_key = (lane & 7) * 16, e_piece = e_key / a.box;
+      const uint8_t* const exps = is_v ? a.c.v_exp : a.c.k_exp;
+      const long long e_sp = is_v ? a.c.ve_sp : a.c.ke_sp, e_sh = is_v ? a.c.ve_sh : a.c.ke_sh;
+      if (lane == 0) {
+        ptx::tma_prefetch_desc(&tm_k);
+        ptx::tma_prefetch_desc(&tm_v);
+      }
+      int n = 0, issued = 0;
+      bool ok = true;
+      for (bool first = true; ok && more; more = walk.next(a, C::kItemCost, s), first = false) {
+        const int* table = a.c.table + (a.prefix_mode ? 0 : s.b) * a.c.table_stride;
+        auto entry = [&](int t) {
+          const int key = a.key_base + t * kTileKeys + lane * a.box;
+          return lane < pieces && key < s.len ? __ldg(table + page_of(a, key)) : 0;
+        };
+        int page = entry(s.t0);
+        if (first) block_sync();
+        for (int t = s.t0; t < s.t1; ++t, ++n) {
+          const int next = t + 1 < s.t1 ? entry(t + 1) : 0;
+          const int key0 = a.key_base + t * kTileKeys, key = key0 + lane * a.box;
+          const bool have = lane < pieces && key < s.len;
+          // A page outside the cache: coordinates that read as zeros, exponents
+          // that say NaN.
+          const bool outside = page < 0 || page >= a.c.num_pages;
+          if (have && outside && a.c.status) atomicOr(a.c.status, FA8_DEVERR_PAGE_RANGE);
+          const int coord = outside ? 0x7fffffff : page;
+          const int slot = key - page_of(a, key) * a.c.page_size;
+          const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, have)) * a.box * D;
+          const int e_coord = __shfl_sync(0xffffffffu, coord, e_piece);
+          const int e_slot = __shfl_sync(0xffffffffu, slot, e_piece) + e_key - e_piece * a.box;
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const int i = 2 * n + v, st = i % NS;
-          if (lane == 0) {
-            if (i >= NS) ok = wait(&sh.kv_empty[st], ((i / NS) - 1) & 1);
-            if (ok) ptx::mbar_arrive_expect_tx(&sh.kv_full[st], bytes);
-          }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          if (have)
-            ptx::tma_load_4d(smem + st * C::kSlotBytes + lane * a.box * D, v ? &tm_v : &tm_k,
-                             &sh.kv_full[st], 0, slot, s.hk, coord, policy);
-          issued = i + 1;
-          if (v == 0) {
-            // K's place is free: the scores of kSlots / 2 tiles ago are done,
-            // so the tile before that has been read, exponents included.
-            uint8_t* const dst = &sh.exps[n % kExpTiles][is_v][e_key];
-            uint64_t* const bar = &sh.e_full[n % kExpTiles];
-            const bool mine = lane < 16 && key0 + e_key < s.len;
-            if (mine && e_coord == 0x7fffffff) {
-              *reinterpret_cast<uint4*>(dst) = make_uint4(~0u, ~0u, ~0u, ~0u);
-              ptx::mbar_arrive(bar);
-            } else {
-              if (mine)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)),
-                             "l"(exps + e_coord * e_sp + s.hk * e_sh + e_slot)
+          for (int v = 0; v < 2; ++v) {
+            const int i = 2 * n + v, st = i % NS;
+            if (lane == 0) {
+              if (i >= NS) ok = wait(&sh.kv_empty[st], ((i / NS) - 1) & 1);
+              if (ok) ptx::mbar_arrive_expect_tx(&sh.kv_full[st], bytes);
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+            if (have)
+              ptx::tma_load_4d(smem + st * C::kSlotBytes + lane * a.box * D, v ? &tm_v : &tm_k,
+                               &sh.kv_full[st], 0, slot, s.hk, coord, policy);
+            issued = i + 1;
+            if (v == 0) {
+              // K's place is free: the scores of kSlots / 2 tiles ago are done,
+              // so the tile before that has been read, exponents included.
+              uint8_t* const dst = &sh.exps[n % kExpTiles][is_v][e_key];
+              uint64_t* const bar = &sh.e_full[n % kExpTiles];
+              const bool mine = lane < 16 && key0 + e_key < s.len;
+              if (mine && e_coord == 0x7fffffff) {
+                *reinterpret_cast<uint4*>(dst) = make_uint4(~0u, ~0u, ~0u, ~0u);
+                ptx::mbar_arrive(bar);
+              } else {
+                if (mine)
+                  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)),
+                               "l"(exps + e_coord * e_sp + s.hk * e_sh + e_slot)
+                               : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                                 ptx::smem_u32(bar))
                              : "memory");
-              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
-                               ptx::smem_u32(bar))
-                           : "memory");
+              }
             }
           }
+          if (!ok) break;
+          page = next;
         }
-        if (!ok) break;
-        page = next;
       }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (!ok && lane == 0) {
-      // Copies in flight land before the block ends.
-      for (int i = max(0, issued - NS); i < issued; ++i)
-        wait_quietly(&sh.kv_full[i % NS], (i / NS) & 1, a.timeout);
-    }
-  } else if (warp >= C::kQWarp) {
-    // ------------------------------------------------------------ rows and Q
-    // One item ahead of the others: row data, and Q as terms, K-major. Each of
-    // the two warps takes every other batch of rows.
-    constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row; rows at a time
-    constexpr int kHalf = C::kRows / C::kQWarps / kPer;
-    constexpr int kMost = C::kRegsHelp < 80 ? 2 : 4;     // loads in flight
-    constexpr int kBatch = kHalf < kMost ? kHalf : kMost;
-    static_assert(C::kRows % (kPer * kBatch * C::kQWarps) == 0, "whole batches");
-    const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
-    const int me = warp - C::kQWarp;
-    block_sync();
-    for (int k = 0; more; more = walk.next(a, C::kItemCost, s), ++k) {
-      const int buf = k & 1;
-      if (k >= 2 && !wait.warp(&sh.q_free[buf], ((k >> 1) - 1) & 1)) break;
-      auto& rw = sh.rows[buf];
-      const int row0 = s.rt * C::kRows, used = min(C::kRows, rows - row0);
-      // Rows up to a whole step are computed with: zeros.
-      const int filled = (used + C::kStep - 1) / C::kStep * C::kStep;
-      const int cl = lane % kLanes;
-      uint4 xs[kBatch];
-      auto ask = [&](int r0) {
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int r = r0 + u * kPer + lane / kLanes;
-          xs[u] = make_uint4(0, 0, 0, 0);
-          if (r < used) {
-            const Row row(a, s.b, s.hk, row0 + r);
-            xs[u] = __ldg(reinterpret_cast<const uint4*>(
-                              a.q + 2 * (row.b * a.q_sb + row.h * a.q_sh + row.i * a.q_ss)) + cl);
-          }
-        }
-      };
-      ask(me * kPer * kBatch);  // on their way while the row data is made
-      int see = s.len;
-#pragma unroll 1
-      for (int r = me * 32 + lane; r < C::kRows; r += 64) {
-        int lim = s.len, id = -1;
-        long long off = 0;
-        if (r < used) {
-          const Row row(a, s.b, s.hk, row0 + r);
-          int len = s.len;
-          if (a.prefix_mode) {
-            len = __ldg(a.c.seqlens + row.b);
-            if (len > a.c.max_len) len = 0;  // refused: its rows are not joined
-          }
-          lim = max(0, min(s.len, len - a.seqlen_q + row.i + 1));
-          id = (row.b * a.heads + row.h) * a.seqlen_q + row.i;
-          off = a.own_rows ? row.b * a.o_sb + row.h * a.o_sh + row.i * a.o_ss : (long long)id * D;
-        }
-        rw.lim[r] = lim;
-        rw.row_id[r] = id;
-        rw.off[r] = off;
-        see = min(see, lim);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (!ok && lane == 0) {
+        // Copies in flight land before the block ends.
+        for (int i = max(0, issued - NS); i < issued; ++i)
+          wait_quietly(&sh.kv_full[i % NS], (i / NS) & 1);
       }
-      see = __reduce_min_sync(0xffffffffu, see);
-      if (lane == 0) rw.all_see[me] = see;
-#pragma unroll 1
-      for (int r0 = me * kPer * kBatch; r0 < filled; r0 += C::kQWarps * kPer * kBatch) {
-        // Stage by stage over the batch: a warp by itself is as fast as its
-        // chains are side by side.
-        uint32_t top[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const uint32_t m = __vmaxu2(__vmaxu2(xs[u].x & 0x7fff7fffu, xs[u].y & 0x7fff7fffu),
-                                      __vmaxu2(xs[u].z & 0x7fff7fffu, xs[u].w & 0x7fff7fffu));
-          top[u] = max(m & 0xffffu, m >> 16);
-        }
-#pragma unroll
-        for (int o = kLanes / 2; o; o >>= 1) {
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u)
-            top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int r = r0 + u * kPer + lane / kLanes;
-          const uint32_t m = top[u];
-          const bool fine = m < (kBf16 ? 0x7f80u : 0x7c00u);
-          const uint32_t bits =
-              kBf16 ? m << 16
-                    : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
-          // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
-          const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
-          if (cl == 0)
-            rw.mul[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
-                             : __int_as_float(0x7fc00000);
-          const float f = fine ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
-          auto scale2 = [&](uint32_t word) -> uint32_t {
-            float2 v;
-            if (kBf16)
-              v = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
-            else
-              v = __half22float2(*reinterpret_cast<const __half2*>(&word));
-            return fine ? h2(v.x * f, v.y * f) : 0u;
-          };
-          xs[u] = make_uint4(scale2(xs[u].x), scale2(xs[u].y), scale2(xs[u].z), scale2(xs[u].w));
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
+    } else if (warp >= C::kQWarp) {
+      // ------------------------------------------------------------ rows and Q
+      // One item ahead of the others: row data, and Q as terms, K-major. Each of
+      // the two warps takes every other batch of rows.
+      constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row; rows at a time
+      constexpr int kHalf = C::kRows / C::kQWarps / kPer;
+      constexpr int kMost = C::kRegsHelp < 80 ? 2 : 4;     // loads in flight
+      constexpr int kBatch = kHalf < kMost ? kHalf : kMost;
+      static_assert(C::kRows % (kPer * kBatch * C::kQWarps) == 0, "whole batches");
+      const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
+      const int me = warp - C::kQWarp;
+      block_sync();
+      for (int k = 0; more; more = walk.next(a, C::kItemCost, s), ++k) {
+        const int buf = k & 1;
+        if (k >= 2 && !wait.warp(&sh.q_free[buf], ((k >> 1) - 1) & 1)) break;
+        auto& rw = sh.rows[buf];
+        const int row0 = s.rt * C::kRows, used = min(C::kRows, rows - row0);
+        // Rows up to a whole step are computed with: zeros.
+        const int filled = (used + C::kStep - 1) / C::kStep * C::kStep;
+        const int cl = lane % kLanes;
+        uint4 xs[kBatch];
+        auto ask = [&](int r0) {
 #pragma unroll
           for (int u = 0; u < kBatch; ++u) {
             const int r = r0 + u * kPer + lane / kLanes;
-            const uint16_t e0 = e4m3x2_of_h2(xs[u].x), e1 = e4m3x2_of_h2(xs[u].y),
-                           e2 = e4m3x2_of_h2(xs[u].z), e3 = e4m3x2_of_h2(xs[u].w);
-            *reinterpret_cast<uint2*>(q_tiles + (buf * C::NWG + r / RW) * C::kQBytes +
-                                      swz<D>(t * RW + r % RW, cl * 8)) =
-                make_uint2((uint32_t)e0 | ((uint32_t)e1 << 16), (uint32_t)e2 | ((uint32_t)e3 << 16));
-            if (t + 1 < NT)
-              xs[u] = make_uint4(rest(xs[u].x, e0), rest(xs[u].y, e1), rest(xs[u].z, e2),
-                                 rest(xs[u].w, e3));
+            xs[u] = make_uint4(0, 0, 0, 0);
+            if (r < used) {
+              const Row row(a, s.b, s.hk, row0 + r);
+              xs[u] = __ldg(reinterpret_cast<const uint4*>(
+                                a.q + 2 * (row.b * a.q_sb + row.h * a.q_sh + row.i * a.q_ss)) + cl);
+            }
+          }
+        };
+        ask(me * kPer * kBatch);  // on their way while the row data is made
+        int see = s.len;
+#pragma unroll 1
+        for (int r = me * 32 + lane; r < C::kRows; r += 64) {
+          int lim = s.len, id = -1;
+          long long off = 0;
+          if (r < used) {
+            const Row row(a, s.b, s.hk, row0 + r);
+            int len = s.len;
+            if (a.prefix_mode) {
+              len = __ldg(a.c.seqlens + row.b);
+              if (len > a.c.max_len) len = 0;  // refused: its rows are not joined
+            }
+            lim = max(0, min(s.len, len - a.seqlen_q + row.i + 1));
+            id = (row.b * a.heads + row.h) * a.seqlen_q + row.i;
+            off = a.own_rows ? row.b * a.o_sb + row.h * a.o_sh + row.i * a.o_ss : (long long)id * D;
+          }
+          rw.lim[r] = lim;
+          rw.row_id[r] = id;
+          rw.off[r] = off;
+          see = min(see, lim);
+        }
+        see = __reduce_min_sync(0xffffffffu, see);
+        if (lane == 0) rw.all_see[me] = see;
+#pragma unroll 1
+        for (int r0 = me * kPer * kBatch; r0 < filled; r0 += C::kQWarps * kPer * kBatch) {
+          // Stage by stage over the batch: a warp by itself is as fast as its
+          // chains are side by side.
+          uint32_t top[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const uint32_t m = __vmaxu2(__vmaxu2(xs[u].x & 0x7fff7fffu, xs[u].y & 0x7fff7fffu),
+                                        __vmaxu2(xs[u].z & 0x7fff7fffu, xs[u].w & 0x7fff7fffu));
+            top[u] = max(m & 0xffffu, m >> 16);
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o; o >>= 1) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+              top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int r = r0 + u * kPer + lane / kLanes;
+            const uint32_t m = top[u];
+            const bool fine = m < (kBf16 ? 0x7f80u : 0x7c00u);
+            const uint32_t bits =
+                kBf16 ? m << 16
+                      : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+            // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
+            const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
+            if (cl == 0)
+              rw.mul[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
+                               : __int_as_float(0x7fc00000);
+            const float f = fine ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
+            auto scale2 = [&](uint32_t word) -> uint32_t {
+              float2 v;
+              if (kBf16)
+                v = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
+              else
+                v = __half22float2(*reinterpret_cast<const __half2*>(&word));
+              return fine ? h2(v.x * f, v.y * f) : 0u;
+            };
+            xs[u] = make_uint4(scale2(xs[u].x), scale2(xs[u].y), scale2(xs[u].z), scale2(xs[u].w));
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+              const int r = r0 + u * kPer + lane / kLanes;
+              const uint16_t e0 = e4m3x2_of_h2(xs[u].x), e1 = e4m3x2_of_h2(xs[u].y),
+                             e2 = e4m3x2_of_h2(xs[u].z), e3 = e4m3x2_of_h2(xs[u].w);
+              *reinterpret_cast<uint2*>(q_tiles + (buf * C::NWG + r / RW) * C::kQBytes +
+                                        swz<D>(t * RW + r % RW, cl * 8)) =
+                  make_uint2((uint32_t)e0 | ((uint32_t)e1 << 16), (uint32_t)e2 | ((uint32_t)e3 << 16));
+              if (t + 1 < NT)
+                xs[u] = make_uint4(rest(xs[u].x, e0), rest(xs[u].y, e1), rest(xs[u].z, e2),
+                                   rest(xs[u].w, e3));
+            }
+          }
+          ask(r0 + C::kQWarps * kPer * kBatch);
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sh.q_full[buf]);
+      }
+    } else if (warp == C::kMmaWarp) {
+      block_sync();
+      if (lane == 0) {
+        // ------------------------------------------------------------ MMA issuer
+        const uint32_t tmem = sh.tmem;
+        const uint32_t ring = ptx::smem_u32(smem), pb = ptx::smem_u32(p_tiles),
+                       qb = ptx::smem_u32(q_tiles);
+        // One product for all warpgroups: an instruction costs the issuing thread
+        // some 100 clocks whatever its N (one product of values per warpgroup
+        // made this thread the slowest of all: 5000 clocks a tile of 64 rows).
+        constexpr uint32_t idesc_s = ptx::idesc_e4m3_f32(128, C::NWG * C::kN);
+        constexpr uint32_t idesc_o = idesc_tt(128, C::NWG * C::kN);
+        bool ok = true;
+        auto scores = [&](int n, int k, bool first) {  // S^T of tile n, in item k
+          const int i = 2 * n, st = i % NS;
+          if (first) ok = wait(&sh.q_full[k & 1], (k >> 1) & 1);
+          ok = ok && wait(&sh.kv_full[st], (i / NS) & 1);
+          if (n > 0) ok = ok && wait(&sh.s_free, (n - 1) & 1);
+          if (!ok) return;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 32; ++kk)
+            ptx::umma_f8(tmem, ptx::smem_desc_kmajor(ring + st * C::kSlotBytes + kk * 32, D),
+                         ptx::smem_desc_kmajor(qb + (k & 1) * C::NWG * C::kQBytes + kk * 32, D), idesc_s,
+                         kk > 0 ? 1u : 0u);
+          ptx::umma_commit(&sh.s_full);
+          ptx::umma_commit(&sh.kv_empty[st]);
+        };
+        auto values = [&](int n, bool first) {  // O^T += V^T P^T of tile n
+          const int i = 2 * n + 1, st = i % NS;
+          ok = wait(&sh.kv_full[st], (i / NS) & 1);
+          ok = ok && wait(&sh.p_full[n & 1], (n >> 1) & 1);
+          if (!ok) return;
+          ptx::tc_fence_after();
+          const uint32_t p = pb + n % C::kPBufs * C::kPBytes;
+#pragma unroll
+          for (int kk = 0; kk < kTileKeys / 32; ++kk)
+            ptx::umma_f8(tmem + C::NWG * C::kN, desc_v<D>(ring + st * C::kSlotBytes + kk * 32 * D),
+                         desc_p<C::kPitch>(p + kk * 32 * C::kPitch), idesc_o,
+                         first && kk == 0 ? 0u : 1u);
+          ptx::umma_commit(&sh.o_done[n & 1]);
+          ptx::umma_commit(&sh.kv_empty[st]);
+        };
+        // The scores of the next tile, be it the next item's first, are issued
+        // before this tile's values: they are ready when its softmax is done.
+        int n = 0, k = 0;
+        scores(0, 0, true);
+        for (; ok && more; ++k) {
+          const int count = s.t1 - s.t0;
+          for (int j = 0; ok && j < count; ++j, ++n) {
+            if (j + 1 < count) {
+              scores(n + 1, k, false);
+            } else {
+              more = walk.next(a, C::kItemCost, s);
+              if (more) scores(n + 1, k + 1, true);
+            }
+            if (ok) values(n, j == 0);
           }
         }
-        ask(r0 + C::kQWarps * kPer * kBatch);
+        ptx::umma_commit(&sh.drain);
+        wait_quietly(&sh.drain, 0);
       }
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sh.q_full[buf]);
     }
-  } else if (warp == C::kMmaWarp) {
-    block_sync();
-    if (lane == 0) {
-      // ------------------------------------------------------------ MMA issuer
-      const uint32_t tmem = sh.tmem;
-      const uint32_t ring = ptx::smem_u32(smem), pb = ptx::smem_u32(p_tiles),
-                     qb = ptx::smem_u32(q_tiles);
-      // One product for all warpgroups: an instruction costs the issuing thread
-      // some 100 clocks whatever its N (one product of values per warpgroup
-      // made this thread the slowest of all: 5000 clocks a tile of 64 rows).
-      constexpr uint32_t idesc_s = ptx::idesc_e4m3_f32(128, C::NWG * C::kN);
-      constexpr uint32_t idesc_o = idesc_tt(128, C::NWG * C::kN);
-      bool ok = true;
-      auto scores = [&](int n, int k, bool first) {  // S^T of tile n, in item k
-        const int i = 2 * n, st = i % NS;
-        if (first) ok = wait(&sh.q_full[k & 1], (k >> 1) & 1);
-        ok = ok && wait(&sh.kv_full[st], (i / NS) & 1);
-        if (n > 0) ok = ok && wait(&sh.s_free, (n - 1) & 1);
-        if (!ok) return;
-        ptx::tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < D / 32; ++kk)
-          ptx::umma_f8(tmem, ptx::smem_desc_kmajor(ring + st * C::kSlotBytes + kk * 32, D),
-                       ptx::smem_desc_kmajor(qb + (k & 1) * C::NWG * C::kQBytes + kk * 32, D), idesc_s,
-                       kk > 0 ? 1u : 0u);
-        ptx::umma_commit(&sh.s_full);
-        ptx::umma_commit(&sh.kv_empty[st]);
-      };
-      auto values = [&](int n, bool first) {  // O^T += V^T P^T of tile n
-        const int i = 2 * n + 1, st = i % NS;
-        ok = wait(&sh.kv_full[st], (i / NS) & 1);
-        ok = ok && wait(&sh.p_full[n & 1], (n >> 1) & 1);
-        if (!ok) return;
-        ptx::tc_fence_after();
-        const uint32_t p = pb + n % C::kPBufs * C::kPBytes;
-#pragma unroll
-        for (int kk = 0; kk < kTileKeys / 32; ++kk)
-          ptx::umma_f8(tmem + C::NWG * C::kN, desc_v<D>(ring + st * C::kSlotBytes + kk * 32 * D),
-                       desc_p<C::kPitch>(p + kk * 32 * C::kPitch), idesc_o,
-                       first && kk == 0 ? 0u : 1u);
-        ptx::umma_commit(&sh.o_done[n & 1]);
-        ptx::umma_commit(&sh.kv_empty[st]);
-      };
-      // The scores of the next tile, be it the next item's first, are issued
-      // before this tile's values: they are ready when its softmax is done.
-      int n = 0, k = 0;
-      scores(0, 0, true);
-      for (; ok && more; ++k) {
-        const int count = s.t1 - s.t0;
-        for (int j = 0; ok && j < count; ++j, ++n) {
-          if (j + 1 < count) {
-            scores(n + 1, k, false);
-          } else {
-            more = walk.next(a, C::kItemCost, s);
-            if (more) scores(n + 1, k + 1, true);
-          }
-          if (ok) values(n, j == 0);
-        }
-      }
-      ptx::umma_commit(&sh.drain);
-      wait_quietly(&sh.drain, 0, a.timeout);
-    }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     // --------------------------------------------------------------- softmax
@@ -1418,8 +1431,6 @@ Shape shape_for(int64_t rows) {
   if (rows <= 32) return {16, 2};
   return {16, 4};
 }
-int ctas_per_sm(int64_t d, const Shape& s) { return s.nwg > 2 ? 1 : (d == 64 && s.rw == 8 ? 3 : 2); }
-
 constexpr int kSmCount = 148;
 
 // Workspace of one set of items.
@@ -1437,7 +1448,7 @@ Layout layout_of(const fa8_decode_params* p, bool prefix_set, int64_t at) {
   l.shape = shape_for(rows);
   l.row_tiles = (rows + l.shape.tile_rows() - 1) / l.shape.tile_rows();
   l.items = p->cache.heads_kv * l.row_tiles * (prefix_set ? 1 : B);
-  l.grid = (int64_t)kSmCount * ctas_per_sm(D, l.shape);
+  l.grid = (int64_t)kSmCount * resident((int)D, l.shape.rw, l.shape.nwg);
   const int64_t parts = 2 * l.grid * l.shape.tile_rows();
   const bool two = p->prefix_len > 0;
   const int64_t all = B * p->heads * p->seqlen_q;

@@ -295,8 +295,8 @@ int fa8_bwd(const fa8_bwd_params* p, void* workspace, int64_t workspace_bytes, v
  * cache stored [page][slot][head][d] is one with other strides). Every (page,
  * head, slot) of K and of V has an exponent byte, indexed [page][head][slot]
  * with unit slot stride (16-byte aligned, other strides multiples of 16):
- * value = code * 2^(byte - 127); 255 marks a row that
- * held an infinity or a NaN and reads as NaN. Token t of sequence b lies in
+ * value = code * 2^(byte - 127); 255 marks a row that held an infinity or a
+ * NaN and reads as NaN (its codes are zero; no code is NaN). Token t of sequence b lies in
  * slot t % page_size of page page_table[b * table_stride + t / page_size];
  * the sequence holds seqlens[b] tokens. Tables and lengths are read on the
  * device only. page_size: 16, 32, 64 or a multiple of 128.

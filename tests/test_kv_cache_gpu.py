@@ -331,6 +331,52 @@ def test_decode_long_and_many(fa8, lens, Hkv, D):
     assert_attention(got, q, cache, table, lens)
 
 
+def test_decode_many_sequences(fa8):
+    """A thousand short sequences, empty ones among them; pages used twice."""
+    rng = random.Random(4)
+    lens = [rng.choice([0, 1, 5, 16, 17, 40]) for _ in range(1000)]
+    cache = make_cache(fa8, 64, 1, 16, 64)
+    table = torch.randint(0, 64, (1000, 3), dtype=torch.int32, device="cuda")
+    table[::7, 1] = table[::7, 0]  # the same page at two places of a sequence
+    seqlens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = make_q(1000, 2, 1, 64, "bf16")
+    got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+    assert_attention(got, q, cache, table, lens)
+
+
+@pytest.mark.parametrize("D,H,Sq", [(128, 2, 1), (64, 8, 3), (128, 32, 1), (128, 64, 2)])
+def test_decode_wait_that_runs_out(fa8, D, H, Sq):
+    """A limit of one clock: the kernel reports it, ends, and the next call is right."""
+    from ada_cute_fp8_flash_attention_b200 import c_abi
+    lens = [3000, 900]
+    cache = make_cache(fa8, pages_for(lens, 64), 1, 64, D)
+    table, seqlens = make_table(lens, 64, pages_for(lens, 64))
+    q = make_q(2, H, Sq, D, "fp16")
+    want = fa8.flash_attn_fp8_decode(q, cache, table, seqlens)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    p = c_abi.decode_params(cache.k.shape[0], 1, 64, D, 2, table.shape[1], H, Sq)
+    c = p.cache
+    c.k, c.v = cache.k.data_ptr(), cache.v.data_ptr()
+    c.k_exp, c.v_exp = cache.k_exp.data_ptr(), cache.v_exp.data_ptr()
+    c.page_table, c.seqlens, c.status = table.data_ptr(), seqlens.data_ptr(), status.data_ptr()
+    out = torch.zeros_like(q)
+    p.q, p.o = q.data_ptr(), out.data_ptr()
+    size = c_abi.decode_workspace_size(p)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert c_abi.decode(p, ws.data_ptr(), size - 1, stream) == c_abi.FA8_ERR_INVALID_ARG
+    assert c_abi.decode(p, ws.data_ptr() + 16, size, stream) == c_abi.FA8_ERR_INVALID_ARG
+    p.wait_timeout_cycles = 1
+    c_abi.check(c_abi.decode(p, ws.data_ptr(), size, stream))
+    torch.cuda.synchronize()
+    assert int(status) == 1
+    status.zero_()
+    p.wait_timeout_cycles = 0
+    c_abi.check(c_abi.decode(p, ws.data_ptr(), size, stream))
+    torch.cuda.synchronize()
+    assert int(status) == 0 and torch.equal(out, want)
+
+
 def test_decode_long_query(fa8):
     """A chunk of a prompt: more query rows than one block holds."""
     lens = [700, 150, 260]
