@@ -64,6 +64,7 @@ namespace dec {
 
 constexpr int kTileKeys = 128;
 constexpr int kMostItemCost = 8;
+constexpr int kMostWarps = 16;         // that prepare Q, or of the softmax
 constexpr float kRise = 5.f;           // log2 of the rise of a maximum that is let be
 constexpr float kPScale = 8.f;         // 8 p 2^e <= 2^(3 + kRise) < 448
 constexpr float kTerm = 16.f;          // weight of a term over the next
@@ -88,7 +89,11 @@ struct Cfg {
   static constexpr int kRows = RW * NWG;
   static constexpr int kThreads = NWG * 128 + 128;
   static constexpr int kMmaWarp = NWG * 4, kLoadWarp = NWG * 4 + 1, kQWarp = NWG * 4 + 2;
-  static constexpr int kQWarps = 2;
+  // Who prepares an item's rows and Q: two helper warps, an item ahead of the
+  // others; with several warpgroups each its own rows at the item's start,
+  // where two warps took 12000 clocks for 64 rows.
+  static constexpr bool kHelperQ = NWG == 1;
+  static constexpr int kQParts = kHelperQ ? 2 : NWG * 4;  // warps that do
   static constexpr int kN = (NT * RW + 15) / 16 * 16;  // columns of the products
   static constexpr int kStep = NWG == 1 ? RW : 8;     // rows read from TMEM at a time
   // What an item costs a block beside its tiles, in tiles: its rows, its first
@@ -420,7 +425,7 @@ struct __align__(16) Shared {
     int row_id[C::kRows];    // (b * heads + h) * seqlen_q + i; -1: no such row
     int lim[C::kRows];       // keys that the row sees
     long long off[C::kRows]; // where a whole row's result goes, in elements
-    int all_see[C::kQWarps]; // keys that all rows of a Q warp see
+    int all_see[kMostWarps]; // keys that all rows of a warp see
   } rows[2];
   struct Group {
     float neg_m[C::RW];      // minus the running maxima
@@ -467,6 +472,119 @@ __device__ __forceinline__ float warp_sums(float (&v)[N]) {
   return v[0];
 }
 
+// Row data of an item and its Q as terms, K-major: rows first..first+ROWS-1 of
+// its tile by WARPS warps, of which this one is number `me`. Rows beyond the
+// last, up to a whole step, are made zero: they are computed with.
+template <class C, bool kBf16, int ROWS, int WARPS, class Rows>
+__device__ __forceinline__ void prepare_rows(const Args& a, const Seg& s, Rows& rw, uint8_t* q_item,
+                                             int first, int me) {
+  constexpr int D = C::D, NT = C::NT, RW = C::RW;
+  constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row; rows of a warp at a time
+  constexpr int kShare = ROWS / WARPS / kPer;
+  constexpr int kMost = C::kHelperQ && C::kRegsHelp < 80 ? 2 : 4;  // loads in flight
+  constexpr int kBatch = kShare < kMost ? kShare : kMost;
+  static_assert(ROWS % (kPer * kBatch * WARPS) == 0, "whole batches");
+  const int lane = threadIdx.x % 32, cl = lane % kLanes;
+  const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
+  const int row0 = s.rt * C::kRows + first, used = min(ROWS, rows - row0);
+  const int filled = (used + C::kStep - 1) / C::kStep * C::kStep;
+  uint4 xs[kBatch];
+  auto ask = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int r = r0 + u * kPer + lane / kLanes;
+      xs[u] = make_uint4(0, 0, 0, 0);
+      if (r < used) {
+        const Row row(a, s.b, s.hk, row0 + r);
+        xs[u] = __ldg(reinterpret_cast<const uint4*>(
+                          a.q + 2 * (row.b * a.q_sb + row.h * a.q_sh + row.i * a.q_ss)) + cl);
+      }
+    }
+  };
+  ask(me * kPer * kBatch);  // on their way while the row data is made
+  int see = s.len;
+#pragma unroll 1
+  for (int r = me * 32 + lane; r < ROWS; r += 32 * WARPS) {
+    int lim = s.len, id = -1;
+    long long off = 0;
+    if (r < used) {
+      const Row row(a, s.b, s.hk, row0 + r);
+      int len = s.len;
+      if (a.prefix_mode) {
+        len = __ldg(a.c.seqlens + row.b);
+        if (len > a.c.max_len) len = 0;  // refused: its rows are not joined
+      }
+      lim = max(0, min(s.len, len - a.seqlen_q + row.i + 1));
+      id = (row.b * a.heads + row.h) * a.seqlen_q + row.i;
+      off = a.own_rows ? row.b * a.o_sb + row.h * a.o_sh + row.i * a.o_ss : (long long)id * D;
+    }
+    rw.lim[first + r] = lim;
+    rw.row_id[first + r] = id;
+    rw.off[first + r] = off;
+    see = min(see, lim);
+  }
+  see = __reduce_min_sync(0xffffffffu, see);
+  if (lane == 0) rw.all_see[first / ROWS * WARPS + me] = see;
+#pragma unroll 1
+  for (int r0 = me * kPer * kBatch; r0 < filled; r0 += WARPS * kPer * kBatch) {
+    // Stage by stage over the batch: a warp by itself is as fast as its
+    // chains are side by side.
+    uint32_t top[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const uint32_t m = __vmaxu2(__vmaxu2(xs[u].x & 0x7fff7fffu, xs[u].y & 0x7fff7fffu),
+                                  __vmaxu2(xs[u].z & 0x7fff7fffu, xs[u].w & 0x7fff7fffu));
+      top[u] = max(m & 0xffffu, m >> 16);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int r = r0 + u * kPer + lane / kLanes;
+      const uint32_t m = top[u];
+      const bool fine = m < (kBf16 ? 0x7f80u : 0x7c00u);
+      const uint32_t bits =
+          kBf16 ? m << 16
+                : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+      // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
+      const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
+      if (cl == 0)
+        rw.mul[first + r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
+                         : __int_as_float(0x7fc00000);
+      const float f = fine ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
+      auto scale2 = [&](uint32_t word) -> uint32_t {
+        float2 v;
+        if (kBf16)
+          v = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
+        else
+          v = __half22float2(*reinterpret_cast<const __half2*>(&word));
+        return fine ? h2(v.x * f, v.y * f) : 0u;
+      };
+      xs[u] = make_uint4(scale2(xs[u].x), scale2(xs[u].y), scale2(xs[u].z), scale2(xs[u].w));
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int r = r0 + u * kPer + lane / kLanes;
+        const uint16_t e0 = e4m3x2_of_h2(xs[u].x), e1 = e4m3x2_of_h2(xs[u].y),
+                       e2 = e4m3x2_of_h2(xs[u].z), e3 = e4m3x2_of_h2(xs[u].w);
+        *reinterpret_cast<uint2*>(q_item + (first + r) / RW * C::kQBytes +
+                                  swz<D>(t * RW + r % RW, cl * 8)) =
+            make_uint2((uint32_t)e0 | ((uint32_t)e1 << 16), (uint32_t)e2 | ((uint32_t)e3 << 16));
+        if (t + 1 < NT)
+          xs[u] = make_uint4(rest(xs[u].x, e0), rest(xs[u].y, e1), rest(xs[u].z, e2),
+                             rest(xs[u].w, e3));
+      }
+    }
+    ask(r0 + WARPS * kPer * kBatch);
+  }
+}
+
 template <class C, bool kBf16>
 __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -479,6 +597,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
   const int G = gridDim.x, cta = blockIdx.x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  if (warp == C::kLoadWarp && lane == 0) {
+    ptx::tma_prefetch_desc(&tm_k);
+    ptx::tma_prefetch_desc(&tm_v);
+  }
   if (warp == 0) {
     for (int i = lane; i < NS; i += 32) {
       ptx::mbar_init(&sh.kv_full[i], 1);
@@ -486,7 +608,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     }
     if (lane < kExpTiles) ptx::mbar_init(&sh.e_full[lane], 32);
     if (lane < 2) {
-      ptx::mbar_init(&sh.q_full[lane], C::kQWarps);
+      ptx::mbar_init(&sh.q_full[lane], C::kQParts);
       ptx::mbar_init(&sh.q_free[lane], C::NWG * 4);
       ptx::mbar_init(&sh.p_full[lane], C::NWG * 4);
       ptx::mbar_init(&sh.o_done[lane], 1);
@@ -613,10 +735,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       const int e_key = (lane & 7) * 16, e_piece = e_key / a.box;
       const uint8_t* const exps = is_v ? a.c.v_exp : a.c.k_exp;
       const long long e_sp = is_v ? a.c.ve_sp : a.c.ke_sp, e_sh = is_v ? a.c.ve_sh : a.c.ke_sh;
-      if (lane == 0) {
-        ptx::tma_prefetch_desc(&tm_k);
-        ptx::tma_prefetch_desc(&tm_v);
-      }
       int n = 0, issued = 0;
       bool ok = true;
       for (bool first = true; ok && more; more = walk.next(a, C::kItemCost, s), first = false) {
@@ -683,121 +801,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         for (int i = max(0, issued - NS); i < issued; ++i)
           wait_quietly(&sh.kv_full[i % NS], (i / NS) & 1);
       }
+    } else if (warp >= C::kQWarp && !C::kHelperQ) {
+      block_sync();
     } else if (warp >= C::kQWarp) {
       // ------------------------------------------------------------ rows and Q
-      // One item ahead of the others: row data, and Q as terms, K-major. Each of
-      // the two warps takes every other batch of rows.
-      constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row; rows at a time
-      constexpr int kHalf = C::kRows / C::kQWarps / kPer;
-      constexpr int kMost = C::kRegsHelp < 80 ? 2 : 4;     // loads in flight
-      constexpr int kBatch = kHalf < kMost ? kHalf : kMost;
-      static_assert(C::kRows % (kPer * kBatch * C::kQWarps) == 0, "whole batches");
-      const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
       const int me = warp - C::kQWarp;
       block_sync();
       for (int k = 0; more; more = walk.next(a, C::kItemCost, s), ++k) {
         const int buf = k & 1;
         if (k >= 2 && !wait.warp(&sh.q_free[buf], ((k >> 1) - 1) & 1)) break;
-        auto& rw = sh.rows[buf];
-        const int row0 = s.rt * C::kRows, used = min(C::kRows, rows - row0);
-        // Rows up to a whole step are computed with: zeros.
-        const int filled = (used + C::kStep - 1) / C::kStep * C::kStep;
-        const int cl = lane % kLanes;
-        uint4 xs[kBatch];
-        auto ask = [&](int r0) {
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const int r = r0 + u * kPer + lane / kLanes;
-            xs[u] = make_uint4(0, 0, 0, 0);
-            if (r < used) {
-              const Row row(a, s.b, s.hk, row0 + r);
-              xs[u] = __ldg(reinterpret_cast<const uint4*>(
-                                a.q + 2 * (row.b * a.q_sb + row.h * a.q_sh + row.i * a.q_ss)) + cl);
-            }
-          }
-        };
-        ask(me * kPer * kBatch);  // on their way while the row data is made
-        int see = s.len;
-#pragma unroll 1
-        for (int r = me * 32 + lane; r < C::kRows; r += 64) {
-          int lim = s.len, id = -1;
-          long long off = 0;
-          if (r < used) {
-            const Row row(a, s.b, s.hk, row0 + r);
-            int len = s.len;
-            if (a.prefix_mode) {
-              len = __ldg(a.c.seqlens + row.b);
-              if (len > a.c.max_len) len = 0;  // refused: its rows are not joined
-            }
-            lim = max(0, min(s.len, len - a.seqlen_q + row.i + 1));
-            id = (row.b * a.heads + row.h) * a.seqlen_q + row.i;
-            off = a.own_rows ? row.b * a.o_sb + row.h * a.o_sh + row.i * a.o_ss : (long long)id * D;
-          }
-          rw.lim[r] = lim;
-          rw.row_id[r] = id;
-          rw.off[r] = off;
-          see = min(see, lim);
-        }
-        see = __reduce_min_sync(0xffffffffu, see);
-        if (lane == 0) rw.all_see[me] = see;
-#pragma unroll 1
-        for (int r0 = me * kPer * kBatch; r0 < filled; r0 += C::kQWarps * kPer * kBatch) {
-          // Stage by stage over the batch: a warp by itself is as fast as its
-          // chains are side by side.
-          uint32_t top[kBatch];
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const uint32_t m = __vmaxu2(__vmaxu2(xs[u].x & 0x7fff7fffu, xs[u].y & 0x7fff7fffu),
-                                        __vmaxu2(xs[u].z & 0x7fff7fffu, xs[u].w & 0x7fff7fffu));
-            top[u] = max(m & 0xffffu, m >> 16);
-          }
-#pragma unroll
-          for (int o = kLanes / 2; o; o >>= 1) {
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u)
-              top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
-          }
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const int r = r0 + u * kPer + lane / kLanes;
-            const uint32_t m = top[u];
-            const bool fine = m < (kBf16 ? 0x7f80u : 0x7c00u);
-            const uint32_t bits =
-                kBf16 ? m << 16
-                      : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
-            // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
-            const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
-            if (cl == 0)
-              rw.mul[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)
-                               : __int_as_float(0x7fc00000);
-            const float f = fine ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
-            auto scale2 = [&](uint32_t word) -> uint32_t {
-              float2 v;
-              if (kBf16)
-                v = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
-              else
-                v = __half22float2(*reinterpret_cast<const __half2*>(&word));
-              return fine ? h2(v.x * f, v.y * f) : 0u;
-            };
-            xs[u] = make_uint4(scale2(xs[u].x), scale2(xs[u].y), scale2(xs[u].z), scale2(xs[u].w));
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-              const int r = r0 + u * kPer + lane / kLanes;
-              const uint16_t e0 = e4m3x2_of_h2(xs[u].x), e1 = e4m3x2_of_h2(xs[u].y),
-                             e2 = e4m3x2_of_h2(xs[u].z), e3 = e4m3x2_of_h2(xs[u].w);
-              *reinterpret_cast<uint2*>(q_tiles + (buf * C::NWG + r / RW) * C::kQBytes +
-                                        swz<D>(t * RW + r % RW, cl * 8)) =
-                  make_uint2((uint32_t)e0 | ((uint32_t)e1 << 16), (uint32_t)e2 | ((uint32_t)e3 << 16));
-              if (t + 1 < NT)
-                xs[u] = make_uint4(rest(xs[u].x, e0), rest(xs[u].y, e1), rest(xs[u].z, e2),
-                                   rest(xs[u].w, e3));
-            }
-          }
-          ask(r0 + C::kQWarps * kPer * kBatch);
-        }
+        prepare_rows<C, kBf16, C::kRows, 2>(a, s, sh.rows[buf], q_tiles + buf * C::NWG * C::kQBytes, 0,
+                                            me);
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&sh.q_full[buf]);
@@ -856,9 +870,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
               scores(n + 1, k, false);
             } else {
               more = walk.next(a, C::kItemCost, s);
-              if (more) scores(n + 1, k + 1, true);
+              if (more && C::kHelperQ) scores(n + 1, k + 1, true);
             }
             if (ok) values(n, j == 0);
+            // Warpgroups that prepare their rows themselves do so when the
+            // item before is done.
+            if (ok && more && j + 1 == count && !C::kHelperQ) scores(n + 1, k + 1, true);
           }
         }
         ptx::umma_commit(&sh.drain);
@@ -893,8 +910,16 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     bool left = false;
     for (; more; more = walk.next(a, C::kItemCost, s), ++k) {
       const auto& rw = sh.rows[k & 1];
+      if constexpr (!C::kHelperQ) {
+        prepare_rows<C, kBf16, RW, 4>(a, s, sh.rows[k & 1],
+                                      q_tiles + (k & 1) * C::NWG * C::kQBytes, w * RW, wq);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sh.q_full[k & 1]);
+      }
       ok = ok && wait.warp(&sh.q_full[k & 1], (k >> 1) & 1);
-      const int all_see = min(rw.all_see[0], rw.all_see[1]);
+      // Keys that all this warpgroup's rows see.
+      const int all_see = C::kHelperQ ? min(rw.all_see[0], rw.all_see[1]) : rw.all_see[4 * w];
       // Rows that exist: steps without any are not computed.
       const int rows = a.seqlen_q * a.group * (a.prefix_mode ? a.c.batch : 1);
       const int used = min(RW, rows - s.rt * C::kRows - w * RW);
