@@ -16,8 +16,7 @@
 // 128-row operand A,
 //   S^T = K Q^T  (128 keys x rows),   O^T += V^T P^T  (D x rows),
 // with the few query rows along N, where small sizes are cheap. One thread
-// then holds one key: its exponent bytes are two registers, its column of P
-// one or a few 16-byte stores.
+// then holds one key: its two exponent bytes and its row of P^T.
 //
 // Rows to 8 bits. tcgen05 wants Q and P in e4m3 too. A value x is held as
 // terms x = t0 + t1 / 16 + t2 / 256, t0 = rn(x), t1 = rn(16 (x - t0)), ...;
@@ -30,20 +29,42 @@
 //
 // Softmax in base 2 with one running maximum per row, m = max(s + e), e the
 // exponent of v_j: then p = 2^(s - m) enters the sum, and what goes to the
-// product is 2^3 * 2^e * p <= 2^3 whatever the exponents are (times 2^5, the
-// rise of the maximum below which nothing is rescaled). The sum is kept
-// per thread, over its own keys, and joined at the end of a row's keys.
+// product is 8 * 2^e * p <= 8 whatever the exponents are (times 2^5, the rise
+// of a maximum that is let be: nothing is looked at row by row, exchanged or
+// rescaled before one rises further). Half the least step of the last term,
+// 2^-10 / 16 or 2^-10 / 256, is then 2^-17 (bf16) or 2^-21 (fp16) of the row's
+// largest: the floor under small p. The sum is kept per thread, over its own
+// keys, in fp32, and joined at the end of a row's keys.
 //
-// Work. Key tiles of 128 of all (sequence, K/V head, tile of query rows) are
-// numbered through and every block takes an equal run of them, which it finds
-// from the lengths on the device by a scan: any mixture of lengths shares the
-// GPU evenly and nothing is read on the host. A block that holds
-// all of an item's keys writes the result; else it writes its unnormalised
-// sums, and a second kernel, launched early and waiting on the device for the
-// first, joins them (always the same shares: results repeat bit by bit).
+// A block: one or more softmax warpgroups (8 or 16 rows each), a warp that
+// brings tiles, a thread that issues products, two warps that prepare the next
+// item's Q. The scores of tile n + 1 are issued before the values of tile n.
+// Registers go from the helpers to the softmax (setmaxnreg). 8 and 16 rows
+// have two blocks an SM (D = 64 and 8 rows three: its tile is half as large
+// and is gone twice as fast), 32 rows two warpgroups, more rows four in one
+// block, whose products are joint: an instruction costs the issuing thread
+// some 100 clocks whatever its N.
+//
+// Work. Key tiles of 128 of all items (sequence, K/V head, tile of query rows)
+// are numbered through, an item weighing a few tiles for itself, and every
+// block takes an equal run of them, which it finds from the lengths on the
+// device by a scan: any mixture of lengths shares the GPU evenly and nothing is
+// read on the host. A block that holds all of an item's keys writes the result;
+// else it writes its unnormalised sums, and a second kernel, launched early and
+// waiting on the device for the first, joins them (always the same shares:
+// results repeat bit by bit).
 //
 // A shared prefix is one more set of items, whose rows are those of the whole
 // batch: one launch for it, one for what is behind it, one that joins both.
+//
+// Measured on B200 (calls one after another, inputs in turn): 64 sequences of
+// up to 16384 keys, 32 heads on 8, bf16, 1.15 GB of cache: 193 us, 5.95 TB/s,
+// 0.91 of the measured copy rate. One sequence of 131072 keys, 32 heads on 4:
+// 35 us, 3.9 TB/s: some 5 us until the first product and as many from the last
+// to the joined result are what a call costs that is this short. 64 sequences
+// behind 16384 shared keys: 88 us; there the chain of a tile (scores, maximum
+// test, exponentials, terms, values) in front of 64 rows bounds it, about 3000
+// clocks, of which the exponentials take 512.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

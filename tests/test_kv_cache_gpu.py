@@ -11,8 +11,10 @@ w = sum p / max p:
   the largest partial sum (truncating accumulation): ds = D 2^-22 B, which moves
   every p by ds and the quotient by 2 ds A; exp2 and the sum of p in fp32 add
   2^-20 A;
-* small p meet a floor: they are held to 2^-19 of the largest p * 2^e of the row,
-  n 2^-19 vmax / w for n keys of magnitude vmax or less.
+* small p meet a floor: the least step of e4m3 is 2^-9, half of it 2^-10; the last
+  of 2 (bf16) or 3 (fp16) terms weighs 16^-1 or 16^-2, and 1 stands for 8: 2^-17 or
+  2^-21 of the largest p * 2^e of the row, times n keys of magnitude vmax or less,
+  over w.
 lse: ds + 2^-20 (1 + |lse|).
 """
 import math
@@ -257,7 +259,8 @@ def oracle_attention(q, cache, table, lens, scale=None, prefix=0):
         out, lse, A, w, big = ref.attention(q[b].double(), k, v, scale)
         ds = (D * 2.0 ** -22 * big).unsqueeze(-1)
         vmax = float(v.abs().nan_to_num(0).max()) if lens[b] else 0.0
-        floor = (lens[b] * 2.0 ** -19 * vmax / w.clamp(min=1)).unsqueeze(-1)
+        least = 2.0 ** (-21 if q.dtype == torch.float16 else -17)
+        floor = (lens[b] * least * vmax / w.clamp(min=1)).unsqueeze(-1)
         tols.append(u * out.abs() + (u + 2 * ds + 2.0 ** -20) * A + floor)
         ltols.append(ds.squeeze(-1) + 2.0 ** -20 * (1 + lse.abs()))
         outs.append(out)
