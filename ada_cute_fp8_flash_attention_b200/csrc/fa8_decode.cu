@@ -760,14 +760,21 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       bool ok = true;
       for (bool first = true; ok && more; more = walk.next(a, C::kItemCost, s), first = false) {
         const int* table = a.c.table + (a.prefix_mode ? 0 : s.b) * a.c.table_stride;
-        auto entry = [&](int t) {
-          const int key = a.key_base + t * kTileKeys + lane * a.box;
-          return lane < pieces && key < s.len ? __ldg(table + page_of(a, key)) : 0;
+        // Table entries of the item's next 32 pieces, one a lane: one load for 4
+        // to 32 tiles, asked for a batch ahead.
+        auto entries = [&](int piece) {
+          const int key = a.key_base + s.t0 * kTileKeys + (piece + lane) * a.box;
+          return key < min(s.len, a.key_base + s.t1 * kTileKeys) ? __ldg(table + page_of(a, key)) : 0;
         };
-        int page = entry(s.t0);
+        int cur = entries(0), next = entries(32), piece = 0;
         if (first) block_sync();
-        for (int t = s.t0; t < s.t1; ++t, ++n) {
-          const int next = t + 1 < s.t1 ? entry(t + 1) : 0;
+        for (int t = s.t0; t < s.t1; ++t, ++n, piece += pieces) {
+          if (piece == 32) {
+            piece = 0;
+            cur = next;
+            next = entries((t - s.t0) * pieces + 32);
+          }
+          const int page = __shfl_sync(0xffffffffu, cur, (piece + lane) & 31);
           const int key0 = a.key_base + t * kTileKeys, key = key0 + lane * a.box;
           const bool have = lane < pieces && key < s.len;
           // A page outside the cache: coordinates that read as zeros, exponents
@@ -813,7 +820,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             }
           }
           if (!ok) break;
-          page = next;
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
