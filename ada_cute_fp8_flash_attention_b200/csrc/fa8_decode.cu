@@ -447,6 +447,8 @@ struct __align__(16) Shared {
     int lim[C::kRows];       // keys that the row sees
     long long off[C::kRows]; // where a whole row's result goes, in elements
     int all_see[kMostWarps]; // keys that all rows of a warp see
+    Seg seg;                 // the item, and whether it is the block's last
+    int last;                // (written and read where helpers prepare it)
   } rows[2];
   struct Group {
     float neg_m[C::RW];      // minus the running maxima
@@ -719,7 +721,22 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       }
     }
   };
-  if (a.own_rows && threadIdx.x == 0) a.seg[cta] = make_int4(-1, 0, 0, 0);
+  // Says where the parts of the block's item k are, if it begins here: from
+  // this block to that of its last tile. One thread does, from the start on.
+  auto no_parts = [&]() {
+    if (a.own_rows) a.seg[cta] = make_int4(-1, 0, 0, 0);
+  };
+  auto say_parts = [&](const Seg& s, int k) {
+    const bool whole = s.t1 == s.nt;
+    if (s.t0 > 0 || (a.own_rows && whole)) return;
+    const int part = 2 * cta + (k > 0 ? 1 : 0), row = s.hk * a.row_tiles + s.rt;
+    const int last = whole ? cta : shares.block_of(s.end);
+    if (a.own_rows)
+      a.seg[cta] = make_int4(last, s.b, row, part);
+    else
+      a.item[(long long)s.b * per + row] =
+          make_int4(cta, last, part, whole ? kItemFull : kItemParts);
+  };
   // Barriers and TMEM are there for all. Every role comes here when it has
   // asked for its first data.
   auto block_sync = [&]() {
@@ -733,6 +750,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     block_sync();
     if (warp == C::kMmaWarp) ptx::tmem_dealloc(sh.tmem, C::kTmemCols);
     fill_empty(threadIdx.x, C::kThreads);
+    if (threadIdx.x == 0) no_parts();
     if (a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
@@ -834,11 +852,19 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       // ------------------------------------------------------------ rows and Q
       const int me = warp - C::kQWarp;
       block_sync();
-      for (int k = 0; more; more = walk.next(a, C::kItemCost, s), ++k) {
+      const bool speaks = me == 0 && lane == 0;
+      if (speaks) no_parts();
+      for (int k = 0; more; ++k) {
         const int buf = k & 1;
         if (k >= 2 && !wait.warp(&sh.q_free[buf], ((k >> 1) - 1) & 1)) break;
         prepare_rows<C, kBf16, C::kRows, 2>(a, s, sh.rows[buf], q_tiles + buf * C::NWG * C::kQBytes, 0,
                                             me);
+        if (speaks) {
+          sh.rows[buf].seg = s;
+          say_parts(s, k);
+        }
+        more = walk.next(a, C::kItemCost, s);
+        if (speaks) sh.rows[buf].last = !more;
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&sh.q_full[buf]);
@@ -888,21 +914,25 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         };
         // The scores of the next tile, be it the next item's first, are issued
         // before this tile's values: they are ready when its softmax is done.
-        int n = 0, k = 0;
+        int n = 0;
         scores(0, 0, true);
-        for (; ok && more; ++k) {
-          const int count = s.t1 - s.t0;
+        for (int k = 0; ok && more; ++k) {
+          const Seg& now = C::kHelperQ ? sh.rows[k & 1].seg : s;
+          const int count = now.t1 - now.t0;
           for (int j = 0; ok && j < count; ++j, ++n) {
             if (j + 1 < count) {
               scores(n + 1, k, false);
-            } else {
-              more = walk.next(a, C::kItemCost, s);
-              if (more && C::kHelperQ) scores(n + 1, k + 1, true);
+            } else if (C::kHelperQ) {
+              more = !sh.rows[k & 1].last;
+              if (more) scores(n + 1, k + 1, true);
             }
             if (ok) values(n, j == 0);
-            // Warpgroups that prepare their rows themselves do so when the
-            // item before is done.
-            if (ok && more && j + 1 == count && !C::kHelperQ) scores(n + 1, k + 1, true);
+          }
+          // Warpgroups that prepare their rows themselves do so when the item
+          // before is done.
+          if (!C::kHelperQ) {
+            more = walk.next(a, C::kItemCost, s);
+            if (ok && more) scores(n, k + 1, true);
           }
         }
         ptx::umma_commit(&sh.drain);
@@ -935,16 +965,28 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     // A warp whose wait gave up goes on to the next barrier, and all four
     // leave there together.
     bool left = false;
-    for (; more; more = walk.next(a, C::kItemCost, s), ++k) {
+    if (!C::kHelperQ && threadIdx.x == 0) no_parts();
+    for (;; ++k) {
       const auto& rw = sh.rows[k & 1];
-      if constexpr (!C::kHelperQ) {
+      bool last = false;
+      if constexpr (C::kHelperQ) {
+        ok = ok && wait.warp(&sh.q_full[k & 1], (k >> 1) & 1);
+        if (!ok) {  // the two barriers where the other warps leave
+          any_of(true);
+          any_of(true);
+          break;
+        }
+        s = rw.seg;
+        last = rw.last;
+      } else {
         prepare_rows<C, kBf16, RW, 4>(a, s, sh.rows[k & 1],
                                       q_tiles + (k & 1) * C::NWG * C::kQBytes, w * RW, wq);
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&sh.q_full[k & 1]);
+        if (threadIdx.x == 0) say_parts(s, k);
+        ok = ok && wait.warp(&sh.q_full[k & 1], (k >> 1) & 1);
       }
-      ok = ok && wait.warp(&sh.q_full[k & 1], (k >> 1) & 1);
       // Keys that all this warpgroup's rows see.
       const int all_see = C::kHelperQ ? min(rw.all_see[0], rw.all_see[1]) : rw.all_see[4 * w];
       // Rows that exist: steps without any are not computed.
@@ -1167,7 +1209,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         if (lane % kEach == 0) reinterpret_cast<float*>(&g.sum[lane / kEach])[wq] = v;
       }
       if (any_of(!ok)) break;
-      const bool begins = s.t0 == 0, whole = begins && s.t1 == s.nt;
+      const bool whole = s.t0 == 0 && s.t1 == s.nt;
       const int part = 2 * cta + (k > 0 ? 1 : 0);
       // Lane r looks after row r (its maximum is there).
       float inv_lane = 0.f;
@@ -1185,15 +1227,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
           else if (a.lse)
             a.lse[id_lane] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
         }
-      }
-      if (w == 0 && tid == 0 && begins && !(a.own_rows && whole)) {
-        // Says where the item's parts are: from this block to its last tile's.
-        const int last = whole ? cta : shares.block_of(s.end);
-        if (a.own_rows)
-          a.seg[cta] = make_int4(last, s.b, s.hk * a.row_tiles + s.rt, part);
-        else
-          a.item[(long long)s.b * per + s.hk * a.row_tiles + s.rt] =
-              make_int4(cta, last, part, whole ? kItemFull : kItemParts);
       }
       // (Should this wait give up, the next barrier ends the block.)
       ok = ok && wait.warp(&sh.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
@@ -1234,6 +1267,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sh.q_free[k & 1]);
+      if (C::kHelperQ ? last : !walk.next(a, C::kItemCost, s)) break;
     }
   }
 
