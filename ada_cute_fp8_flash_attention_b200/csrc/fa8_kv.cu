@@ -254,10 +254,11 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_row_kernel(const CopyArg
 // token r / heads. The tokens' places are found once, by one thread each; then
 // every thread keeps the rows of a batch of K and V in flight together.
 template <int D, bool kBf16, bool kWrite>
-__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const CopyArgs a) {
+__global__ void __launch_bounds__(kCopyThreads, kWrite ? 8 : 1) kv_copy_kernel(const CopyArgs a) {
   constexpr int kLanes = D / 8, kGroups = kCopyThreads / kLanes;
   // Rows of K and of V that a thread has asked for: 2, 4, 8 took 88, 91, 119 us
-  // (write) and 70, 68, 83 us (read) for 65000 tokens of 8 heads.
+  // (write) and 70, 68, 83 us (read) for 65000 and 55000 tokens of 8 heads; with
+  // eight blocks an SM the write takes 84, the read 80.
   constexpr int kRowsInFlight = kWrite ? 2 : 4;
   __shared__ Place places[kMostTokens];
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
