@@ -238,9 +238,9 @@ def flash_attn_fp8_shared_prefix(q, cache, page_table, seqlens, prefix_len, soft
     """``flash_attn_fp8_decode`` for a batch whose sequences begin with the same tokens.
 
     The first ``prefix_len`` tokens (a host number, any value a table row can hold)
-    are read once for the whole batch, from the pages of ``page_table``'s row 0, and
-    all the batch's queries meet them together; the other rows' entries for whole
-    prefix pages are not read. The result is that of ``flash_attn_fp8_decode`` up to
+    are taken from the pages of ``page_table``'s row 0 (the other rows' entries for
+    whole prefix pages are not read), and all the batch's queries meet them together;
+    a prefix too short for that to pay is met by each sequence for itself. The result is that of ``flash_attn_fp8_decode`` up to
     the order of its sums, given that every row's first prefix_len tokens hold what
     row 0's hold. Sequences shorter than the prefix see their own length of it.
     """

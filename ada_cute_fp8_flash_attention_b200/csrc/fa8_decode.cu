@@ -55,7 +55,8 @@
 // results repeat bit by bit).
 //
 // A shared prefix is one more set of items, whose rows are those of the whole
-// batch: one launch for it, one for what is behind it, one that joins both.
+// batch: one launch for it, one for what is behind it, one that joins both. A
+// prefix of few tiles is left in each sequence's own items (prefix_apart).
 //
 // Measured on B200 (calls one after another, inputs in turn): 64 sequences of
 // up to 16384 keys, 32 heads on 8, bf16, 1.15 GB of cache: 193 us, 5.95 TB/s,
@@ -190,6 +191,7 @@ struct Args {
   int key0;          // first key of these items
   int key_base;      // key0 rounded down to where a TMA box may start
   int prefix_len;
+  int shared_pages;  // table columns that every sequence has in row 0
   int row_tiles;     // tiles of query rows per (sequence, K/V head)
   int box;           // keys of a TMA box: min(page_size, 128)
   Divisor by_page, by_group, by_seq_rows, by_row_tiles;  // (by_seq_rows: group * seqlen_q)
@@ -782,7 +784,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         // to 32 tiles, asked for a batch ahead.
         auto entries = [&](int piece) {
           const int key = a.key_base + s.t0 * kTileKeys + (piece + lane) * a.box;
-          return key < min(s.len, a.key_base + s.t1 * kTileKeys) ? __ldg(table + page_of(a, key)) : 0;
+          if (key >= min(s.len, a.key_base + s.t1 * kTileKeys)) return 0;
+          const int col = page_of(a, key);
+          return __ldg((col < a.shared_pages ? a.c.table : table) + col);
         };
         int cur = entries(0), next = entries(32), piece = 0;
         if (first) block_sync();
@@ -1527,6 +1531,22 @@ struct Layout {
 };
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
+// Whether a prefix has a set of items of its own. Three launches in a row take
+// 16 us however little there is to do, two 10; met by every sequence for
+// itself (from the same pages, in L2) the prefix is more tiles to each block.
+// Together / one by one, us, 32 heads on 8, D = 128, 296 blocks: 16 sequences
+// behind 1024 (3.5 tiles a block) 24 / 17, behind 2048 (7) 26 / 21, 32 behind
+// 2048 (14) 29 / 31, 64 behind 2048 (28) 40 / 51; 16 heads of D = 64, 444
+// blocks: 8 behind 1000 (2.3) 21 / 15, 48 behind 1024 (14) 30 / 39.
+bool prefix_apart(const fa8_decode_params* p) {
+  if (p->prefix_len == 0) return false;
+  const int64_t rows = p->seqlen_q * (p->heads / p->cache.heads_kv);
+  const Shape s = shape_for(rows);
+  const int64_t tiles = (rows + s.tile_rows() - 1) / s.tile_rows() * p->cache.batch *
+                        p->cache.heads_kv * ((p->prefix_len + kTileKeys - 1) / kTileKeys);
+  return tiles > 10 * kSmCount * resident((int)p->cache.head_dim, s.rw, s.nwg);
+}
+
 Layout layout_of(const fa8_decode_params* p, bool prefix_set, int64_t at) {
   Layout l;
   const int64_t D = p->cache.head_dim, B = p->cache.batch;
@@ -1536,7 +1556,7 @@ Layout layout_of(const fa8_decode_params* p, bool prefix_set, int64_t at) {
   l.items = p->cache.heads_kv * l.row_tiles * (prefix_set ? 1 : B);
   l.grid = (int64_t)kSmCount * resident((int)D, l.shape.rw, l.shape.nwg);
   const int64_t parts = 2 * l.grid * l.shape.tile_rows();
-  const bool two = p->prefix_len > 0;
+  const bool two = prefix_apart(p);
   const int64_t all = B * p->heads * p->seqlen_q;
   l.part_o = at;
   l.part_ml = l.part_o + up256(parts * D * 4);
@@ -1614,9 +1634,10 @@ int run_set(const fa8_decode_params* p, Args a, const Layout& l, char* ws, int d
 template <int D, bool kBf16>
 int run(const fa8_decode_params* p, Args a, char* ws, int dev, cudaStream_t stream) {
   cudaError_t e;
-  if (p->prefix_len == 0) {
+  if (!prefix_apart(p)) {
     const Layout l = layout_of(p, false, 0);
     a.own_rows = 1;
+    a.shared_pages = (int)(p->prefix_len / p->cache.page_size);
     const int st = run_set<D, kBf16>(p, a, l, ws, dev, stream);
     if (st) return st;
     a.row_tiles = (int)l.row_tiles;
@@ -1686,7 +1707,7 @@ int64_t fa8_decode_workspace_size(const fa8_decode_params* p) {
     return -1;
   }
   if (p->cache.batch == 0 || p->heads == 0 || p->seqlen_q == 0) return 0;
-  if (p->prefix_len == 0) return layout_of(p, false, 0).end;
+  if (!prefix_apart(p)) return layout_of(p, false, 0).end;
   return layout_of(p, false, layout_of(p, true, 0).end).end;
 }
 

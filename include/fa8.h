@@ -369,9 +369,10 @@ int fa8_kv_read(const fa8_kv_copy_params* p, void* stream);
  * key give o = 0 and lse = -inf.
  *
  * prefix_len > 0: the first prefix_len tokens of all sequences are the same
- * and are read once for the whole batch, from the pages of row 0 of the
- * table (the caller vouches for it; no other row's pages are read for them).
- * The result is that of prefix_len = 0.
+ * (the caller vouches for it). Whole pages of them are taken from row 0 of the
+ * table alone, and all the batch's queries meet the prefix together where that
+ * is faster than each sequence by itself (the rule goes by sizes). The result
+ * is that of prefix_len = 0 up to the order of its sums.
  *
  * The caller provides fa8_decode_workspace_size() bytes of device workspace,
  * 256-byte aligned; nothing in it is kept or expected between calls, and

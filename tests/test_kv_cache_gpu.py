@@ -560,6 +560,37 @@ def test_shared_prefix_many_rows(fa8):
     assert_attention(got, q, cache, table, lens, prefix=prefix)
 
 
+@pytest.mark.parametrize("B,H,Hkv,Sq,D,prefix,dtype", [
+    (64, 16, 16, 1, 64, 1000, "fp16"), (48, 32, 8, 1, 128, 1100, "bf16"),
+    (40, 32, 2, 1, 128, 5000, "fp16"), (20, 8, 8, 3, 64, 4100, "bf16"),
+    (3, 64, 1, 1, 64, 65537, "bf16")])
+def test_shared_prefix_apart(fa8, B, H, Hkv, Sq, D, prefix, dtype):
+    """Prefixes long enough that they are met by all queries together."""
+    ps = 64
+    lens = [prefix + Sq + (11 * b) % 140 for b in range(B)]
+    lens[1] = prefix - 3  # inside the prefix
+    if B > 10:
+        lens[5], lens[7] = 0, prefix
+    table, seqlens, pages = shared_table(lens, prefix, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    same_prefix(cache, table, lens, prefix)
+    q = make_q(B, H, Sq, D, dtype, size=0.7)
+    got = fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix, return_lse=True)
+    assert_attention(got, q, cache, table, lens, prefix=0)
+    bad = table.clone()
+    bad[1:, :prefix // ps] = -5
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    same = fa8.flash_attn_fp8_shared_prefix(q, cache, bad, seqlens, prefix, status=status)
+    assert torch.equal(same, got[0]) and int(status) == 0
+    seqlens[2] = table.shape[1] * ps + 1  # refused: left as it was, the others served
+    out = torch.full_like(q, 5.0)
+    fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix, out=out, status=status)
+    assert int(status) == 4 and bool((out[2] == 5).all())
+    keep = [b for b in range(B) if b != 2]
+    tol = 4 * torch.finfo(q.dtype).eps * (got[0].abs() + 1)
+    assert bool(((out - got[0]).abs() <= tol)[keep].all())
+
+
 def test_shared_prefix_edges(fa8):
     """Sequences inside the prefix, empty ones, no prefix, nothing behind it."""
     prefix, ps = 200, 16
