@@ -58,14 +58,14 @@
 // batch: one launch for it, one for what is behind it, one that joins both. A
 // prefix of few tiles is left in each sequence's own items (prefix_apart).
 //
-// Measured on B200 (calls one after another, inputs in turn): 64 sequences of
-// up to 16384 keys, 32 heads on 8, bf16, 1.15 GB of cache: 193 us, 5.95 TB/s,
-// 0.91 of the measured copy rate. One sequence of 131072 keys, 32 heads on 4:
-// 35 us, 3.9 TB/s: some 5 us until the first product and as many from the last
-// to the joined result are what a call costs that is this short. 64 sequences
-// behind 16384 shared keys: 88 us; there the chain of a tile (scores, maximum
-// test, exponentials, terms, values) in front of 64 rows bounds it, about 3000
-// clocks, of which the exponentials take 512.
+// Measured on B200 (replayed from a graph, inputs in turn): 64 sequences of up
+// to 16384 keys, 32 heads on 8, bf16, 1.15 GB of cache: 176 us, 6.5 TB/s, the
+// measured copy rate. One sequence of 131072 keys, 32 heads on 4: 32 us, 4.2
+// TB/s: some 5 us until the first product and as many from the last to the
+// joined result are what a call costs that is this short. 64 sequences behind
+// 16384 shared keys: 86 us; there the chain of a tile (scores, maximum test,
+// exponentials, terms, values) in front of 64 rows bounds it, about 3000 clocks,
+// of which the exponentials take 512.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
