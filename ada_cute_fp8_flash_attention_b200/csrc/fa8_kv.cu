@@ -119,7 +119,7 @@ __device__ __forceinline__ Place place_of(const CopyArgs& a, int tok) {
     b = lo;
     const int c0 = __ldg(a.cu + b), c1 = __ldg(a.cu + b + 1);
     if (tok < c0 || tok >= c1) return p;  // before the first or behind the last sequence
-    n = c1 - c0;
+    n = (int)((unsigned)c1 - (unsigned)c0);
     back = c1 - tok;
     p.k = tok * a.k_ss;
     p.v = tok * a.v_ss;
@@ -132,7 +132,7 @@ __device__ __forceinline__ Place place_of(const CopyArgs& a, int tok) {
     p.v = b * a.v_sb + i * a.v_ss;
   }
   const int len = __ldg(a.c.seqlens + b);
-  if (len > a.c.max_len || len < n) {
+  if (len > a.c.max_len || len < n || n < 0) {  // (n wraps if cu[0] is far below 0)
     if (a.c.status) atomicOr(a.c.status, FA8_DEVERR_VARLEN_RANGE);
     return p;
   }

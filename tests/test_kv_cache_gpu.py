@@ -241,6 +241,24 @@ def test_copy_status_bits(fa8):
     assert bool(k[3, :, 2].isnan().all()) and not bool(k[3, :, :2].isnan().any())
 
 
+def test_copy_first_offset_far_below_zero(fa8):
+    """cu[1] - cu[0] does not fit 32 bits: refused, nothing is written on either side."""
+    cache = make_cache(fa8, 4, 2, 16, 64)
+    before = clone(cache)
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+    seqlens = torch.tensor([2], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([-2**31, 10], dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.randn(10, 2, 64, device="cuda").half()
+    fa8.kv_cache_write(cache, x, x, table, seqlens, cu, status=status)
+    assert int(status) == 4
+    assert all(torch.equal(u8(t), u8(o)) for t, o in zip(cache, before))
+    status.zero_()
+    out = tuple(torch.full((10, 2, 64), 9.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    k, v = fa8.kv_cache_read(cache, table, seqlens, cu, 10, out=out, status=status)
+    assert int(status) == 4 and bool((k == 9).all()) and bool((v == 9).all())
+
+
 # ------------------------------------------------------------------ attention
 
 def oracle_attention(q, cache, table, lens, scale=None, prefix=0):
