@@ -226,7 +226,7 @@ def flash_attn_fp8_decode(q, cache, page_table, seqlens, softmax_scale=None, ret
     evenly. ``status`` (optional int32 device tensor) bits: 4 = a sequence whose
     length does not fit its table row, left unwritten; 8 = a page id outside the
     cache, its sequence's queries that see it are NaN; 1 = a wait inside the kernel
-    gave up.
+    gave up. For serving: nothing is recorded for a backward pass.
     """
     res = _C.flash_attn_fp8_decode(q, cache[0], cache[1], cache[2], cache[3], page_table, seqlens,
                                    0, softmax_scale, return_lse, out, status)
@@ -240,9 +240,10 @@ def flash_attn_fp8_shared_prefix(q, cache, page_table, seqlens, prefix_len, soft
     The first ``prefix_len`` tokens (a host number, any value a table row can hold)
     are taken from the pages of ``page_table``'s row 0 (the other rows' entries for
     whole prefix pages are not read), and all the batch's queries meet them together;
-    a prefix too short for that to pay is met by each sequence for itself. The result is that of ``flash_attn_fp8_decode`` up to
-    the order of its sums, given that every row's first prefix_len tokens hold what
-    row 0's hold. Sequences shorter than the prefix see their own length of it.
+    a prefix too short for that to pay is met by each sequence for itself. The result
+    is that of ``flash_attn_fp8_decode`` up to the order of its sums, given that every
+    row's first prefix_len tokens hold what row 0's hold. Sequences shorter than the
+    prefix see their own length of it.
     """
     res = _C.flash_attn_fp8_decode(q, cache[0], cache[1], cache[2], cache[3], page_table, seqlens,
                                    int(prefix_len), softmax_scale, return_lse, out, status)

@@ -537,7 +537,7 @@ __device__ __forceinline__ void prepare_rows(const Args& a, const Seg& s, Rows& 
       int len = s.len;
       if (a.prefix_mode) {
         len = __ldg(a.c.seqlens + row.b);
-        if (len > a.c.max_len) len = 0;  // refused: its rows are not joined
+        if (len < 0 || len > a.c.max_len) len = 0;  // refused: its rows are not joined
       }
       lim = max(0, min(s.len, len - a.seqlen_q + row.i + 1));
       id = (row.b * a.heads + row.h) * a.seqlen_q + row.i;
@@ -711,11 +711,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       if (len < 0 || tiles_of(a, len) > 0) continue;
       if (a.own_rows) {
         const int n = a.heads * a.seqlen_q;
-        for (int j = first; j < n * (D / 8); j += step) {
-          const int row = j / (D / 8), h = row / a.seqlen_q, i = row - h * a.seqlen_q;
-          reinterpret_cast<uint4*>(a.o + 2 * (b * a.o_sb + h * a.o_sh + i * a.o_ss))[j % (D / 8)] =
+        const int piece = first % (D / 8);
+        for (int row = first / (D / 8); row < n; row += step / (D / 8)) {
+          const int h = row / a.seqlen_q, i = row - h * a.seqlen_q;
+          reinterpret_cast<uint4*>(a.o + 2 * (b * a.o_sb + h * a.o_sh + i * a.o_ss))[piece] =
               make_uint4(0, 0, 0, 0);
-          if (a.lse && j % (D / 8) == 0) a.lse[(long long)b * n + row] = -INFINITY;
+          if (a.lse && piece == 0) a.lse[(long long)b * n + row] = -INFINITY;
         }
       } else {
         for (int j = first; j < per; j += step)
@@ -1397,7 +1398,7 @@ struct Set {
   const float2* full_ml;
   const float* part_o;
   const float2* part_ml;
-  int row_tiles, tile_rows;
+  int row_tiles, tile_rows, grid;
 };
 
 // Joins every row's prefix with what is behind it; a warp per row.
@@ -1416,7 +1417,10 @@ __global__ void __launch_bounds__(128, 4) prefix_join_kernel(const Args a, const
                            row / s.tile_rows);
     if (it.w == kItemFull) {
       sum.add(s.full_o, s.full_ml, 1, [&](int) { return (long long)id; });
-    } else if (it.w == kItemParts) {
+    } else if (it.w == kItemParts && it.x >= 0 && it.x <= it.y && it.y < s.grid && it.z >= 0 &&
+               it.z < 2 * s.grid) {
+      // (A block that gave up waiting has not said where its later items are:
+      // the workspace holds anything there.)
       sum.add(s.part_o, s.part_ml, it.y - it.x + 1, [&](int k) {
         return (long long)(k == 0 ? it.z : 2 * (it.x + k)) * s.tile_rows + row % s.tile_rows;
       });
@@ -1670,6 +1674,7 @@ int run(const fa8_decode_params* p, Args a, char* ws, int dev, cudaStream_t stre
       s.part_ml = reinterpret_cast<const float2*>(ws + l.part_ml);
       s.row_tiles = (int)l.row_tiles;
       s.tile_rows = l.shape.tile_rows();
+      s.grid = (int)l.grid;
       return s;
     };
     const int64_t rows = p->cache.batch * p->heads * p->seqlen_q;

@@ -398,6 +398,55 @@ def test_decode_wait_that_runs_out(fa8, D, H, Sq):
     assert int(status) == 0 and torch.equal(out, want)
 
 
+def test_prefix_wait_that_runs_out(fa8):
+    """Blocks that give up have not said where all their items are: whatever the
+    workspace holds there, the joining kernel stays inside it."""
+    from ada_cute_fp8_flash_attention_b200 import c_abi
+    B, H, D, ps, prefix = 64, 16, 64, 64, 1000
+    lens = [prefix + 1 + (11 * b) % 140 for b in range(B)]
+    table, seqlens, pages = shared_table(lens, prefix, ps)
+    cache = make_cache(fa8, pages, H, ps, D, spread=0.3)
+    same_prefix(cache, table, lens, prefix)
+    q = make_q(B, H, 1, D, "fp16")
+    want = fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    p = c_abi.decode_params(pages, H, ps, D, B, table.shape[1], H, 1)
+    c = p.cache
+    c.k, c.v = cache.k.data_ptr(), cache.v.data_ptr()
+    c.k_exp, c.v_exp = cache.k_exp.data_ptr(), cache.v_exp.data_ptr()
+    c.page_table, c.seqlens, c.status = table.data_ptr(), seqlens.data_ptr(), status.data_ptr()
+    out = torch.zeros_like(q)
+    p.q, p.o, p.prefix_len = q.data_ptr(), out.data_ptr(), prefix
+    size = c_abi.decode_workspace_size(p)
+    assert size % 16 == 0
+    ws = torch.empty(size // 4, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    for places in ((2**31 - 1, 2**31 - 1, 2**31 - 1), (0, 2**31 - 1, 0), (-5, 3, -9), (7, 2, 0)):
+        ws.view(-1, 4)[:] = torch.tensor(places + (2,), dtype=torch.int32, device="cuda")
+        status.zero_()
+        p.wait_timeout_cycles = 1
+        c_abi.check(c_abi.decode(p, ws.data_ptr(), size, stream))
+        torch.cuda.synchronize()
+        assert int(status) == 1
+        status.zero_()
+        p.wait_timeout_cycles = 0
+        c_abi.check(c_abi.decode(p, ws.data_ptr(), size, stream))
+        torch.cuda.synchronize()
+        assert int(status) == 0 and torch.equal(out, want)
+
+
+def test_decode_many_rows_without_keys(fa8):
+    """More 16-byte pieces of results than 31 bits count, all of them zeros."""
+    H, Sq = 2056, 65535
+    cache = make_cache(fa8, 1, 8, 16, 128)
+    table, seqlens = make_table([0], 16, 1, width=1)
+    q = make_q(1, 1, 1, 128, "fp16").expand(1, H, Sq, 128)
+    out = torch.full((1, H, Sq, 128), 3.0, dtype=torch.float16, device="cuda")
+    fa8.flash_attn_fp8_decode(q, cache, table, seqlens, out=out)
+    bits = out.view(torch.int32)
+    assert int(bits.amax()) == 0 and int(bits.amin()) == 0
+
+
 def test_decode_long_query(fa8):
     """A chunk of a prompt: more query rows than one block holds."""
     lens = [700, 150, 260]
