@@ -846,8 +846,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      if (!ok && lane == 0) {
-        // Copies in flight land before the block ends.
+      if (lane == 0) {
+        // Copies in flight land before the block ends, whoever gave up waiting:
+        // a share that fits the ring never makes this warp wait, so it does not
+        // learn of it. When nobody did they have landed, and this is at once.
         for (int i = max(0, issued - NS); i < issued; ++i)
           wait_quietly(&sh.kv_full[i % NS], (i / NS) & 1);
       }
