@@ -257,6 +257,14 @@ __device__ __forceinline__ bool wait_bar_abort(uint64_t* bar, uint32_t parity, l
   return true;
 }
 
+// What is in flight when a CTA ends: waited for up to the default limit, not
+// the caller's, which may be shorter than a copy takes.
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!ptx::mbar_try_wait(bar, parity) && clock64() - t0 < kTimeout) {
+  }
+}
+
 template <int D, bool kDq>
 __global__ void __launch_bounds__(kThreadsTile, 1)
     bwd_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -359,17 +367,9 @@ __global__ void __launch_bounds__(kThreadsTile, 1)
         ++issued;
       }
       // Copies still in flight must land before the CTA exits (bounded waits).
-      for (int t = max(0, issued - 2); t < issued; ++t) {
-        const long long t0 = clock64();
-        while (!ptx::mbar_try_wait(&bars.ld_full[t & 1], (uint32_t)(t >> 1) & 1u) &&
-               clock64() - t0 < p.timeout) {
-        }
-      }
-      {
-        const long long t0 = clock64();
-        while (!ptx::mbar_try_wait(&bars.fixed_full, 0) && clock64() - t0 < p.timeout) {
-        }
-      }
+      for (int t = max(0, issued - 2); t < issued; ++t)
+        drain_wait(&bars.ld_full[t & 1], (uint32_t)(t >> 1) & 1u);
+      drain_wait(&bars.fixed_full, 0);
     }
   } else if (warp == kMmaWarp) {
     if (lane == 0 && n_iter > 0) {
@@ -434,9 +434,7 @@ __global__ void __launch_bounds__(kThreadsTile, 1)
       }
       ptx::umma_commit(&bars.acc_done);
       // Drain: every product issued here completes before TMEM is freed.
-      const long long t0 = clock64();
-      while (!ptx::mbar_try_wait(&bars.acc_done, 0) && clock64() - t0 < p.timeout) {
-      }
+      drain_wait(&bars.acc_done, 0);
     }
   } else {
     // ------------------------------------------------------ elementwise warps

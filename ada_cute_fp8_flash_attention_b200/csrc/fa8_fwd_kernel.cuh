@@ -250,6 +250,13 @@ __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity,
   }
 }
 
+// What is in flight when a CTA ends: waited for up to the default limit.
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!ptx::mbar_try_wait(bar, parity) && clock64() - t0 < kTimeoutCycles) {
+  }
+}
+
 // Position of K(t) / V(t) (t-th K/V tile processed, of n) in the load order
 // K0, K1, V0, K2, V1, ..., K(n-1), V(n-2), V(n-1) — the order in which the
 // products use them (S(t+1) is issued before O += P(t) V(t)).
@@ -632,21 +639,12 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks)
                            pol_kv);
         ++issued;
       }
-      if (!ok) {
-        // Drain: wait (bounded) for the last copies issued so that no TMA
-        // write lands in shared memory after this CTA exits.
-        for (int L = max(0, issued - NS); L < issued; ++L) {
-          const long long t0 = clock64();
-          while (!ptx::mbar_try_wait(&bars.kv_full[L % NS], (L / NS) & 1) &&
-                 clock64() - t0 < p.timeout_cycles) {
-          }
-        }
-      }
-      {
-        const long long t0 = clock64();
-        while (!ptx::mbar_try_wait(&bars.q_full, 0) && clock64() - t0 < p.timeout_cycles) {
-        }
-      }
+      // Drain: the last copies issued land before this CTA exits, whoever gave
+      // up waiting (a loader whose tiles fit the ring never waits itself, and in
+      // an ordinary CTA they have landed). Bounded, but not by the caller's
+      // limit, which may be shorter than a copy takes.
+      for (int L = max(0, issued - NS); L < issued; ++L) drain_wait(&bars.kv_full[L % NS], (L / NS) & 1);
+      drain_wait(&bars.q_full, 0);
     } else if (warp == kMmaWarp && lane == 0) {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t q_addr = s_base + C::kOffQ;
@@ -729,9 +727,7 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks)
       }
       // Drain every MMA this thread issued before TMEM is freed.
       ptx::umma_commit(&bars.drain);
-      const long long t0 = clock64();
-      while (!ptx::mbar_try_wait(&bars.drain, 0) && clock64() - t0 < p.timeout_cycles) {
-      }
+      drain_wait(&bars.drain, 0);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
