@@ -747,16 +747,19 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks)
     float m_run = -INFINITY;  // running max of s*scale*log2e
     float l_run = 0.f;
     bool ok = true;
-    // PV(j) complete: phase j >> 1 of o_done[j & 1].
-    auto wait_pv = [&](int j) -> bool {
-      return bounded_wait(&bars.o_done[j & 1], (j >> 1) & 1, abort_flag, p.status,
-                          p.timeout_cycles);
+    // One answer for the whole warp: lanes may differ where a limit runs out just
+    // as the phase completes, and the TMEM accesses behind a wait take all of them.
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu,
+                        bounded_wait(bar, parity, abort_flag, p.status, p.timeout_cycles));
     };
+    // PV(j) complete: phase j >> 1 of o_done[j & 1].
+    auto wait_pv = [&](int j) -> bool { return wait_warp(&bars.o_done[j & 1], (j >> 1) & 1); };
 
     for (int tl = 0; tl < n && ok; ++tl) {
       const int kv = kv_top - tl;
       if (lane == 0) FA8_TR(warp, tl, 0);
-      ok = bounded_wait(&bars.s_full, tl & 1, abort_flag, p.status, p.timeout_cycles);
+      ok = wait_warp(&bars.s_full, tl & 1);
       if (lane == 0) FA8_TR(warp, tl, 1);
       if (!ok) break;
       ptx::tc_fence_after();
@@ -889,13 +892,11 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks)
       if (lane == 0) ptx::mbar_arrive(&bars.p_full[tl & 1]);
       if (lane == 0) FA8_TR(warp, tl, 5);
     }
-    ok = __all_sync(0xffffffffu, ok);
 
     // Epilogue: O / l -> global, LSE.
     if (lane == 0) FA8_TR(warp, 62, 2);
     if (ok) ok = wait_pv(n - 1);
     if (lane == 0) FA8_TR(warp, 62, 3);
-    ok = __all_sync(0xffffffffu, ok);
     // One CTA-wide verdict for the four softmax warps (the TMA-store path
     // below has a barrier that all of them must reach).
     if (!ok && lane == 0) softmax_fail_sh = 1;

@@ -107,3 +107,40 @@ def test_varlen_out_of_range_sequence_is_refused_in_kernel(abi, cuda):
     o = out.float().cpu().numpy()
     assert np.all(o[16:] == 7.0), "the refused sequence must be left unwritten"
     assert np.all(o[:16] == 0.0)
+
+
+@pytest.mark.parametrize("D,Sq,Skv,causal", [(128, 256, 256, 0), (128, 300, 1008, 1),
+                                             (64, 128, 384, 0), (64, 1008, 1008, 1),
+                                             (128, 1, 5008, 0)])
+def test_limit_of_one_clock_beside_another_stream(abi, cuda, D, Sq, Skv, causal):
+    """Waits that run out at any place, in warps whose lanes may differ, in CTAs whose
+    loads fit the ring: reported, and nothing lands in the calls beside and after."""
+    import torch
+    B, H, Hkv = 2, 4, 2
+    q, k, v = U.inputs(B, H, Hkv, Sq, Skv, D, "normal", seed=6)
+    qd, kd, vd = (U.to_dev(x, cuda) for x in (q, k, v))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    outs = [torch.zeros((B, H, Sq, D), dtype=torch.float16, device=cuda) for _ in range(22)]
+    o_ref, _ = U.oracle(q, k, v, causal=bool(causal), q_offset=Skv - Sq if causal else 0)
+
+    def call(out, limit, stream):
+        p = abi.params(B, H, Hkv, Sq, Skv, D)
+        p.q, p.k, p.v, p.o = qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), out.data_ptr()
+        p.causal, p.q_offset = causal, Skv - Sq if causal else 0
+        if limit:
+            p.status, p.wait_timeout_cycles = status.data_ptr(), limit
+        abi.check(abi.fwd(p, stream.cuda_stream))
+
+    here, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    call(outs[0], 0, here)
+    torch.cuda.synchronize()
+    for out in outs[2:]:
+        call(outs[1], 1, here)
+        call(out, 0, side)
+    torch.cuda.synchronize()
+    assert int(status.item()) == 1
+    assert all(torch.equal(o, outs[0]) for o in outs[2:])
+    call(outs[1], 0, here)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[1], outs[0])
+    U.assert_close(outs[0].float().cpu().numpy(), o_ref)
