@@ -289,6 +289,20 @@ __device__ __forceinline__ uint32_t swz(int row, int col) {
   return (uint32_t)(row * kPitch + ((chunk ^ x) << 4) + (col & 15));
 }
 
+// Are all codes of row `row` of a tile of D bytes a row zero? (A swizzle moves
+// pieces of 16 bytes within their row; the rows of a warp start at different ones.)
+template <int D>
+__device__ __forceinline__ bool zero_row(const uint8_t* tile, int row) {
+  uint32_t any = 0;
+#pragma unroll 1
+  for (int c = 0; c < D / 16; ++c) {
+    const int piece = (c + row * D / 128) % (D / 16);
+    const uint4 x = *reinterpret_cast<const uint4*>(tile + row * D + piece * 16);
+    any |= x.x | x.y | x.z | x.w;
+  }
+  return (any & 0x7f7f7f7fu) == 0;
+}
+
 // Instruction descriptor of O^T += V^T P^T: both operands MN-major.
 __host__ __device__ constexpr uint32_t idesc_tt(int m, int n) {
   return ptx::idesc_e4m3_f32(m, n, true) | (1u << 15);
@@ -1015,7 +1029,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         ok = ok && wait.warp(&sh.e_full[n % kExpTiles], (n / kExpTiles) & 1);
         const int kb = sh.exps[n % kExpTiles][0][tid], vb = sh.exps[n % kExpTiles][1][tid];
         const float kf = kv::exp_factor(kb);
-        const float vexp = vb == kv::kExpNan ? 0.f : (float)(vb - kv::kExpBias);
+        float vexp = vb == kv::kExpNan ? 0.f : (float)(vb - kv::kExpBias);
         const float vf = dead ? 0.f : kv::exp_factor(vb) * kPScale;
 
         ok = ok && wait.warp(&sh.s_full, n & 1);
@@ -1081,6 +1095,16 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         // buffer the product of the tile before has to be waited for.
         if (C::kPBufs == 1 && n > 0) ok = ok && wait.warp(&sh.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
         if (rise) {
+          // A row of zeros has the exponent of 1 whatever its neighbours have. It
+          // adds nothing under any exponent, and as one of 1 it would be the
+          // maximum of keys whose values are small, whose terms then vanish: the
+          // least one. Looked at only where it could set a maximum.
+          const bool look = vb == kv::kExpBias && !dead && (t == s.t0 || high + vexp > kRise);
+          if (__any_sync(0xffffffffu, look)) {
+            const int st = (2 * n + 1) % NS;
+            ok = ok && wait.warp(&sh.kv_full[st], ((2 * n + 1) / NS) & 1);
+            if (look && zero_row<D>(smem + st * C::kSlotBytes, tid)) vexp = (float)kv::kMinExp;
+          }
           float top = -INFINITY;
 #pragma unroll
           for (int r = 0; r < RW; r += 2) {

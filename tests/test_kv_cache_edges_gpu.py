@@ -1,12 +1,26 @@
 """GPU checks of the cache's attention where it can go wrong: calls whose waits run
-out beside calls of another stream.
+out beside calls of another stream; value rows of zeros.
 
-Helpers, oracle and the tolerances of plain cases are those of test_kv_cache_gpu.
+Tolerances, with u = eps / 2 of q's type (2^-11 fp16, 2^-8 bf16), p the weights, w
+their sum, c_j the codes and 2^e_j the factor of value row j:
+* the result is rounded once: u |o|, or half a subnormal step where that is more
+  (fp16 values below 2^-14 are multiples of 2^-24: 2^-25); p is rounded once: u A,
+  A = sum p |v| / w;
+* scores: fp32 sums of D products, each addition off by 2^-22 of the largest partial
+  sum B, and q's elements by half the least step of the last term: ds = D 2^-22 B +
+  2^-21 (bf16) or 2^-25 (fp16) of the row's largest |q| times the largest scale *
+  sum |k| of a key. It moves the quotient by 2 ds A. exp2 and sums: 2^-20 A;
+* small p meet a floor, 2^-17 or 2^-21 of the row's largest p_j 2^e_j over rows j
+  that are not zero, for every key: that times sum_j |c_j| / w.
+lse: ds + 2^-20 (1 + |lse|). A result beyond the type's largest is infinite.
 """
+import math
 
 import pytest
 
-from tests.test_kv_cache_gpu import (make_cache, make_q, make_table, pages_for)
+from oracle import kv_cache_ref as ref
+from tests.test_kv_cache_gpu import (E4M3, make_cache, make_q, make_table, pages_for,
+                                     same_prefix, shared_table, u8)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -16,6 +30,60 @@ pytestmark = pytest.mark.gpu
 def fa8(cuda):
     import ada_cute_fp8_flash_attention_b200 as m
     return m
+
+
+def held(codes_u8, exps, row, n):
+    """float64 code values (H_kv, n, D) and exponents (H_kv, n) of a sequence's tokens."""
+    pos = torch.arange(n, device="cuda")
+    page, slot = row.long()[pos // codes_u8.shape[2]], pos % codes_u8.shape[2]
+    codes = ref.decode_e4m3(codes_u8[page, :, slot]).transpose(0, 1)
+    return codes, exps[page, :, slot].transpose(0, 1).double() - 127
+
+
+def assert_near(got, q, cache, table, lens, scale=None):
+    """Output and lse against 64 bits, by the bounds at the head of this file."""
+    out, lse = got
+    B, H, Sq, D = q.shape
+    G = H // cache.k.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    fp16 = q.dtype == torch.float16
+    info = torch.finfo(q.dtype)
+    u, top, least = info.eps / 2, info.max, info.smallest_normal * info.eps / 2
+    for b, n in enumerate(lens):
+        kc, ke = held(u8(cache.k), cache.k_exp, table[b], n)
+        vc, ve = held(u8(cache.v), cache.v_exp, table[b], n)
+        k, c, e = (x.repeat_interleave(G, 0) for x in (kc * torch.exp2(ke).unsqueeze(-1), vc, ve))
+        v = c * torch.exp2(e).unsqueeze(-1)
+        for i in range(Sq):
+            m = n - Sq + i + 1
+            if m <= 0:
+                assert bool((out[b, :, i] == 0).all()) and bool((lse[b, :, i] == -math.inf).all())
+                continue
+            x = q[b, :, i].double()
+            s = torch.einsum("hd,hnd->hn", x, k[:, :m]) * scale
+            mag = torch.einsum("hd,hnd->hn", x.abs(), k[:, :m].abs()) * scale
+            ks = k[:, :m].abs().sum(-1).amax(-1) * scale
+            ds = D * 2.0 ** -22 * mag.amax(-1) + x.abs().amax(-1) * 2.0 ** (-25 if fp16 else -21) * ks
+            p = torch.exp(s - s.amax(-1, keepdim=True))
+            w = p.sum(-1)
+            want = torch.einsum("hn,hnd->hd", p, v[:, :m]) / w[:, None]
+            A = torch.einsum("hn,hnd->hd", p, v[:, :m].abs()) / w[:, None]
+            solid = (c[:, :m] != 0).any(-1)
+            # in logs: p may be less than a double holds and 2^e as large
+            lead = torch.where(solid, s / math.log(2) + e[:, :m], -math.inf).amax(-1)
+            lead = torch.exp2(lead - torch.logsumexp(s, -1) / math.log(2))
+            floor = lead[:, None] * c[:, :m].abs().sum(1) * 2.0 ** (-21 if fp16 else -17)
+            tol = (u * want.abs()).clamp(min=least) + (u + 2 * ds[:, None] + 2.0 ** -20) * A + floor
+            err = (out[b, :, i].double() - want).abs()
+            far = want.abs() > top  # may round to the largest or to infinity
+            bad = (~(err <= tol)) & ~far
+            assert not bool(bad.any()), \
+                f"out: {float(err[bad].max()):.3g} over {float(tol[bad].min()):.3g}"
+            wlse = torch.logsumexp(s, -1)
+            ltol = ds + 2.0 ** -20 * (1 + wlse.abs())
+            lerr = (lse[b, :, i].double() - wlse).abs()
+            assert bool((lerr <= ltol).all()), \
+                f"lse: {float(lerr.max()):.3g} over {float(ltol.min()):.3g}"
 
 
 def c_decode(cache, table, seqlens, q, out, status=None, prefix=0, lse=None):
@@ -67,3 +135,62 @@ def test_waits_that_run_out_beside_another_stream(fa8, D, Hkv, G, n):
     c_abi.check(c_abi.decode(p, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def put_row(cache, table, page_size, b, pos, k=None, v=None):
+    """Token `pos` of sequence b gets these K and V rows (H_kv, D), float64."""
+    page, slot = int(table[b, pos // page_size]), pos % page_size
+    for name, x in (("k", k), ("v", v)):
+        if x is not None:
+            values, byte = ref.quantise(x)
+            u8(getattr(cache, name))[page, :, slot] = u8(values.float().to(E4M3))
+            getattr(cache, name + "_exp")[page, :, slot] = byte
+
+
+def toward(q, score, heads_kv):
+    """A key (H_kv, D) whose score with the mean query row of each group is `score`."""
+    D = q.shape[-1]
+    x = q.double().view(heads_kv, -1, D).mean(1)
+    return x * (score * D ** 0.5 / (x * x).sum(-1, keepdim=True))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("size", [1.0, 0.1, 1e-3])
+@pytest.mark.parametrize("D,H,Hkv,Sq,where", [(128, 8, 2, 1, 0), (64, 4, 4, 3, 200),
+                                              (128, 32, 1, 2, 511), (128, 64, 1, 2, 130)])
+def test_decode_row_of_zeros(fa8, D, H, Hkv, Sq, where, size, dtype):
+    """A value row of zeros under the top score leaves the others' precision alone."""
+    lens, ps = [512, 512, 40], 16
+    pages = pages_for(lens, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    values, byte = ref.quantise(cache.v.double() * ref.factor(cache.v_exp).unsqueeze(-1) * size)
+    cache = cache._replace(v=values.float().to(E4M3), v_exp=byte)
+    table, seqlens = make_table(lens, ps, pages)
+    q = make_q(3, H, Sq, D, dtype, size=1.0)
+    zero = torch.zeros(Hkv, D, dtype=torch.float64, device="cuda")
+    for b, pos in ((0, where), (1, 5), (1, where), (2, 36)):
+        put_row(cache, table, ps, b, pos, toward(q[b], 8.0, Hkv), zero)
+    u8(cache.v)[int(table[1, 0]), :, 5] = 128  # minus zeros
+    got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+    assert_near(got, q, cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("size", [1.0, 0.1, 1e-3])
+def test_shared_prefix_row_of_zeros(fa8, size, dtype):
+    D, H, Hkv, ps, prefix, B = 128, 32, 8, 16, 1040, 48
+    lens = [prefix + 1 + (7 * b) % 50 for b in range(B)]
+    table, seqlens, pages = shared_table(lens, prefix, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    values, byte = ref.quantise(cache.v.double() * ref.factor(cache.v_exp).unsqueeze(-1) * size)
+    cache = cache._replace(v=values.float().to(E4M3), v_exp=byte)
+    same_prefix(cache, table, lens, prefix)
+    q = make_q(B, H, 1, D, dtype, size=1.0)
+    zero = torch.zeros(Hkv, D, dtype=torch.float64, device="cuda")
+    put_row(cache, table, ps, 0, 0, toward(q[0], 8.0, Hkv), zero)
+    put_row(cache, table, ps, 0, 777, toward(q[3], 8.0, Hkv), zero)
+    put_row(cache, table, ps, 5, lens[5] - 1, toward(q[5], 9.0, Hkv), zero)
+    before = fa8.launch_count()
+    got = fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix, return_lse=True)
+    assert fa8.launch_count() - before == 3  # the prefix has a launch of its own
+    assert_near(got, q, cache, table, lens)
