@@ -28,13 +28,20 @@
 // to 11 (fp16) or 8 (bf16) bits, as it would be for a 16-bit product.
 //
 // Softmax in base 2 with one running maximum per row, m = max(s + e), e the
-// exponent of v_j: then p = 2^(s - m) enters the sum, and what goes to the
-// product is 8 * 2^e * p <= 8 whatever the exponents are (times 2^5, the rise
-// of a maximum that is let be: nothing is looked at row by row, exchanged or
-// rescaled before one rises further). Half the least step of the last term,
-// 2^-10 / 16 or 2^-10 / 256, is then 2^-17 (bf16) or 2^-21 (fp16) of the row's
-// largest: the floor under small p. The sum is kept per thread, over its own
-// keys, in fp32, and joined at the end of a row's keys.
+// exponent of v_j over a reference, the largest of the item's first tile: then
+// p = 2^(s - m) enters the sum, and what goes to the product is 8 * 2^e * p <= 8
+// whatever the exponents are (times 2^5, the rise of a maximum that is let be:
+// nothing is looked at row by row, exchanged or rescaled before one rises
+// further). Half the least step of the last term, 2^-10 / 16 or 2^-10 / 256, is
+// then 2^-17 (bf16) or 2^-21 (fp16) of the row's largest: the floor under small
+// p. The sum is kept per thread, over its own keys, in fp32, and joined at the
+// end of a row's keys.
+//
+// p is as far from 1 as e is from 0. Within 2^24 the sum keeps its digits. Where
+// a key's exponent is further away, or a row of zeros (whose exponent says
+// nothing) has a score so high that it would set the maximum, the block computes
+// its share once more in fp32 when it is done (share_again): values of any size
+// beside each other are right, at a price that others do not pay.
 //
 // A block: one or more softmax warpgroups (8 or 16 rows each), a warp that
 // brings tiles, a thread that issues products, two warps that prepare the next
@@ -86,9 +93,12 @@ namespace dec {
 
 constexpr int kTileKeys = 128;
 constexpr int kMostItemCost = 8;
+constexpr int kAgainBar = 6;           // named barrier of share_again
 constexpr int kMostWarps = 16;         // that prepare Q, or of the softmax
 constexpr float kRise = 5.f;           // log2 of the rise of a maximum that is let be
-constexpr float kPScale = 8.f;         // 8 p 2^e <= 2^(3 + kRise) < 448
+constexpr int kPShift = 3;             // 8 p 2^e <= 2^(3 + kRise) < 448
+constexpr float kWide = 24.f;          // how far exponents of V may be from the item's reference
+constexpr int kLeastRef = -100;        // least reference exponent
 constexpr float kTerm = 16.f;          // weight of a term over the next
 constexpr long long kTimeout = 4000000000LL;
 constexpr int kWaitHintNs = 20000;
@@ -141,7 +151,7 @@ struct Cfg {
   static constexpr int kCtas = resident(D, RW, NWG);
   // 227 KB a block, 228 KB an SM of which each block takes 1 KB and its
   // static variables; 1 KB to align.
-  static constexpr int kStatic = 2688 + 80 * kRows;
+  static constexpr int kStatic = 2736 + 80 * kRows + 16 * NWG;
   static constexpr int kBudget = (kCtas == 1 ? 227 : (228 - kCtas) / kCtas) * 1024 - kStatic - 1024;
   // P in two buffers where four tiles of the ring still fit beside them: the
   // next one is then written while the product of this one runs.
@@ -317,6 +327,18 @@ __device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
   return d;
 }
 
+// l = 2^k * x with 1 <= x < 2 for normal l; a NaN is its own x.
+__device__ __forceinline__ int log2_below(float l) { return (__float_as_int(l) >> 23 & 255) - 127; }
+__device__ __forceinline__ float over_log2(float l, int k) {
+  return l != l ? l : __int_as_float(__float_as_int(l) - k * (1 << 23));
+}
+// ln(2^m l), l > 0 (or NaN): its exponent is added to m first, so that a maximum
+// that is far from the largest score costs no digits.
+__device__ __forceinline__ float ln_of(float m, float l) {
+  const int k = log2_below(l);
+  return ((m + (float)k) + log2f(over_log2(l, k))) * 0.6931471805599453f;
+}
+
 __device__ __forceinline__ float sum_of(const float4& v) { return (v.x + v.y) + (v.z + v.w); }
 
 // P^T as operand B: rows (keys) of kPitch bytes; columns beyond them are in the
@@ -457,6 +479,8 @@ struct __align__(16) Shared {
   uint64_t drain;
   uint32_t tmem;
   int abort;
+  int again;                 // an item's exponents of V are too far apart
+  Walk start;                // where the block's share begins
   struct __align__(16) Rows {  // of an item; read four at a time
     float mul[C::kRows];     // scale * log2(e) * the power of two of the row of Q
     int row_id[C::kRows];    // (b * heads + h) * seqlen_q + i; -1: no such row
@@ -471,6 +495,7 @@ struct __align__(16) Shared {
     float step[C::RW];       // and what the last rise added to that
     float4 sum[C::RW];       // the four warps' sums of a row
     float4 top[C::RW];       // and maxima of a tile
+    float4 e_max;            // the four warps' largest exponents of V in a first tile
   } g[C::NWG];
   static_assert(sizeof(Rows) % 16 == 0 && sizeof(Group) % 16 == 0, "read four at a time");
   static_assert(C::kSlots / 2 + 2 <= kExpTiles,
@@ -624,6 +649,221 @@ __device__ __forceinline__ void prepare_rows(const Args& a, const Seg& s, Rows& 
   }
 }
 
+// The values of four codes.
+__device__ __forceinline__ void floats_of(uint32_t w, float (&x)[4]) {
+  const uint32_t h0 = ptx::cvt_e4m3x2_to_f16x2((uint16_t)w),
+                 h1 = ptx::cvt_e4m3x2_to_f16x2((uint16_t)(w >> 16));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)),
+               b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+  x[0] = a.x;
+  x[1] = a.y;
+  x[2] = b.x;
+  x[3] = b.y;
+}
+
+// A block's share once more, by its softmax warps, in fp32 and straight from the
+// cache: for items whose values are so different in size that one reference does
+// not serve them (kWide). Four rows at a time; a warp takes every W-th run of 32
+// keys, a lane a key for the scores and D / 32 columns for the values. The
+// maximum of s is the weights' reference, that of s + e the sum of values', so
+// neither leaves the range of fp32. A call whose every share is computed again
+// takes six to eight times as long (64 sequences of up to 16384 keys 1190 us), 15
+// times behind a shared prefix. Kept apart from the loop over tiles: as a branch
+// of it, with a second exponential for P, it cost every call 10 to 17 %.
+template <class C, bool kBf16>
+__device__ __forceinline__ void share_again(const Args& a, Walk walk, float* scratch) {
+  constexpr int D = C::D, W = C::NWG * 4, R = 4, V = D / 32;
+  static_assert((R * D + 3 * W * R + W * R * D) * 4 <= C::kSlots * C::kSlotBytes, "scratch in the ring");
+  float* const q_s = scratch;           // [R][D]
+  float* const ms_s = q_s + R * D;      // [W][R] of each warp: maximum of s,
+  float* const me_s = ms_s + W * R;     // of s + e,
+  float* const l_s = me_s + W * R;      // sum,
+  float* const o_s = l_s + W * R;       // [W][R][D] and sums of values
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const kv::CacheView& c = a.c;
+  const int rows = a.seqlen_q * a.group * (a.prefix_mode ? c.batch : 1);
+  Seg s;
+  for (int k = 0; walk.next(a, C::kItemCost, s); ++k) {
+    const int used = min(C::kRows, rows - s.rt * C::kRows);
+    const bool whole = s.t0 == 0 && s.t1 == s.nt;
+    const int part = 2 * blockIdx.x + (k > 0 ? 1 : 0);
+    const int first = max(a.key0, a.key_base + s.t0 * kTileKeys);
+    const int last = min(s.len, a.key_base + s.t1 * kTileKeys);
+    const int* const table = c.table + (a.prefix_mode ? 0 : s.b) * c.table_stride;
+#pragma unroll 1
+    for (int r0 = 0; r0 < used; r0 += R) {
+      ptx::named_barrier_sync(kAgainBar, W * 32);  // the scratch is free
+#pragma unroll 1
+      for (int i = threadIdx.x; i < R * D; i += W * 32) {
+        const int r = r0 + i / D;
+        float x = 0.f;
+        if (r < used) {
+          const Row row(a, s.b, s.hk, s.rt * C::kRows + r);
+          const unsigned short w = __ldg(reinterpret_cast<const unsigned short*>(a.q) +
+                                         row.b * a.q_sb + row.h * a.q_sh + row.i * a.q_ss + i % D);
+          x = kBf16 ? __uint_as_float((uint32_t)w << 16) : __half2float(__ushort_as_half(w));
+        }
+        q_s[i] = x;
+      }
+      int lim[R];
+      float ms[R], me[R], l[R], o[R][V];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        lim[r] = 0;
+        if (r0 + r < used) {
+          const Row row(a, s.b, s.hk, s.rt * C::kRows + r0 + r);
+          const int len = a.prefix_mode ? __ldg(c.seqlens + row.b) : s.len;
+          if (len >= 0 && len <= c.max_len) lim[r] = min(last, len - a.seqlen_q + row.i + 1);
+        }
+        ms[r] = me[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[r][v] = 0.f;
+      }
+      ptx::named_barrier_sync(kAgainBar, W * 32);
+#pragma unroll 1
+      for (int key0 = first + warp * 32; key0 < last; key0 += W * 32) {
+        const int key = key0 + lane;
+        const uint8_t *kr = nullptr, *vr = nullptr;
+        int kb = kv::kExpNan, vb = kv::kExpNan;
+        if (key < last) {
+          const int col = page_of(a, key), slot = key - col * c.page_size;
+          const long long page = __ldg((col < a.shared_pages ? c.table : table) + col);
+          if (page >= 0 && page < c.num_pages) {
+            kr = c.k + page * c.k_sp + s.hk * c.k_sh + slot * c.k_ss;
+            vr = c.v + page * c.v_sp + s.hk * c.v_sh + slot * c.v_ss;
+            kb = c.k_exp[page * c.ke_sp + s.hk * c.ke_sh + slot];
+            vb = c.v_exp[page * c.ve_sp + s.hk * c.ve_sh + slot];
+          }
+        }
+        float y[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) y[r] = 0.f;
+        if (kr) {
+#pragma unroll 1
+          for (int d = 0; d < D; d += 16) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(kr + d));
+            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float f[4];
+              floats_of(words[i], f);
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+                const float4 q4 = *reinterpret_cast<const float4*>(q_s + r * D + d + 4 * i);
+                y[r] = fmaf(q4.x, f[0], fmaf(q4.y, f[1], fmaf(q4.z, f[2], fmaf(q4.w, f[3], y[r]))));
+              }
+            }
+          }
+        }
+        const float kf = kv::exp_factor(kb), e = (float)(vb - kv::kExpBias);
+        uint32_t any = 1;
+        if (vr && vb == kv::kExpBias) {
+          any = 0;
+#pragma unroll 1
+          for (int d = 0; d < D; d += 4)
+            any |= __ldg(reinterpret_cast<const uint32_t*>(vr + d)) & 0x7f7f7f7fu;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float sc = key < lim[r] ? y[r] * a.scale_log2 * kf : -INFINITY;
+          const float t = any && vb != kv::kExpNan ? sc + e : -INFINITY;
+          const float m_new = fmaxf(ms[r], warp_max(sc)), e_new = fmaxf(me[r], warp_max(t));
+          const float m_use = m_new == -INFINITY ? 0.f : m_new, e_use = e_new == -INFINITY ? 0.f : e_new;
+          l[r] = l[r] * ptx::ex2(ms[r] - m_use) + ptx::ex2(sc - m_use);
+          const float f = ptx::ex2(me[r] - e_use);
+#pragma unroll
+          for (int v = 0; v < V; ++v) o[r][v] *= f;
+          y[r] = sc == -INFINITY         ? 0.f
+                 : vb == kv::kExpNan ? __int_as_float(0x7fc00000)
+                                     : ptx::ex2(t - e_use);
+          ms[r] = m_new;
+          me[r] = e_new;
+        }
+#pragma unroll 4
+        for (int kk = 0; kk < 32; ++kk) {
+          const uint8_t* const row =
+              reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)vr, kk));
+          uint32_t w = 0;
+          if (row)
+            w = V == 4 ? __ldg(reinterpret_cast<const uint32_t*>(row) + lane)
+                       : __ldg(reinterpret_cast<const unsigned short*>(row) + lane);
+          float x[4];
+          floats_of(w, x);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float yr = __shfl_sync(0xffffffffu, y[r], kk);
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[r][v] = fmaf(yr, x[v], o[r][v]);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 16; i; i >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], i);
+        const int at = warp * R + r;
+        if (lane == 0) {
+          ms_s[at] = ms[r];
+          me_s[at] = me[r];
+          l_s[at] = l[r];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) o_s[at * D + lane * V + v] = o[r][v];
+      }
+      ptx::named_barrier_sync(kAgainBar, W * 32);
+      const int r = r0 + warp;
+      if (warp < R && r < used) {  // a warp joins a row
+        float m = -INFINITY, e = -INFINITY, sum = 0.f, x[V];
+        for (int w = 0; w < W; ++w) {
+          m = fmaxf(m, ms_s[w * R + warp]);
+          e = fmaxf(e, me_s[w * R + warp]);
+        }
+        const float m_use = m == -INFINITY ? 0.f : m, e_use = e == -INFINITY ? 0.f : e;
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = 0.f;
+        for (int w = 0; w < W; ++w) {
+          const int at = w * R + warp;
+          sum = fmaf(ptx::ex2(ms_s[at] - m_use), l_s[at], sum);
+          const float f = ptx::ex2(me_s[at] - e_use);
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[v] = fmaf(f, o_s[at * D + lane * V + v], x[v]);
+        }
+        // times 2^(e - m), in two steps for the range of fp32
+        const float by = e == -INFINITY ? 0.f : e - m_use, here = fminf(fmaxf(by, -100.f), 100.f);
+        const float f0 = sum == 0.f ? 0.f : ptx::ex2(here) / sum, f1 = ptx::ex2(by - here);
+        const float top = sum == 0.f ? -INFINITY : m;
+        const Row row(a, s.b, s.hk, s.rt * C::kRows + r);
+        const long long id = (row.b * a.heads + row.h) * a.seqlen_q + row.i;
+        const long long at = (long long)part * C::kRows + r;
+        if (lane == 0) {
+          if (!whole)
+            a.part_ml[at] = make_float2(top, sum);
+          else if (!a.own_rows)
+            a.full_ml[id] = make_float2(top, sum);
+          else if (a.lse)
+            a.lse[id] = sum == 0.f ? -INFINITY : ln_of(top, sum);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float out = x[v] * f0 * f1;
+          const int d = lane * V + v;
+          if (!whole)
+            a.part_o[at * D + d] = out;
+          else if (!a.own_rows)
+            a.full_o[id * D + d] = out;
+          else if (kBf16)
+            reinterpret_cast<__nv_bfloat16*>(a.o)[row.b * a.o_sb + row.h * a.o_sh + row.i * a.o_ss + d] =
+                __float2bfloat16(out);
+          else
+            reinterpret_cast<__half*>(a.o)[row.b * a.o_sb + row.h * a.o_sh + row.i * a.o_ss + d] =
+                __float2half(out);
+        }
+      }
+    }
+  }
+}
+
 template <class C, bool kBf16>
 __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -656,7 +896,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       ptx::mbar_init(&sh.s_full, 1);
       ptx::mbar_init(&sh.s_free, C::NWG * 4);
       ptx::mbar_init(&sh.drain, 1);
-      sh.abort = 0;
+      sh.abort = sh.again = 0;
     }
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
@@ -716,6 +956,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     }
   }
 
+  if (threadIdx.x == 0) sh.start = walk;
+
   // Sequences without a key among these items have no tile and no block of
   // their own: their rows (items) are filled in by block b mod G.
   auto fill_empty = [&](int first, int step) {
@@ -760,6 +1002,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
+  };
+  auto end_sync = [&]() {
+    __syncwarp();
+    ptx::tc_fence_before();
+    __syncthreads();
   };
   Seg s;
   bool more = walk.next(a, C::kItemCost, s);
@@ -960,6 +1207,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         wait_quietly(&sh.drain, 0);
       }
     }
+    end_sync();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     // --------------------------------------------------------------- softmax
@@ -1017,8 +1265,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
 #pragma unroll
       for (int r = 0; r < RW / 2; ++r) l2[r] = 0;
       // Running maximum of row `lane`. A row that sees any of this block's keys
-      // of the item sees some of the first tile: that one sets it.
+      // of the item sees some of the first tile: that one sets it, and the
+      // reference that exponents of V are taken over, its largest.
       float m_lane = 0.f;
+      int ref = 0;
       if (lane < RW) g.neg_m[lane] = 0.f;  // (every warp writes the same)
       __syncwarp();
       for (int t = s.t0; t < s.t1; ++t, ++n) {
@@ -1029,8 +1279,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         ok = ok && wait.warp(&sh.e_full[n % kExpTiles], (n / kExpTiles) & 1);
         const int kb = sh.exps[n % kExpTiles][0][tid], vb = sh.exps[n % kExpTiles][1][tid];
         const float kf = kv::exp_factor(kb);
-        float vexp = vb == kv::kExpNan ? 0.f : (float)(vb - kv::kExpBias);
-        const float vf = dead ? 0.f : kv::exp_factor(vb) * kPScale;
+        const bool first = t == s.t0, v_nan = !dead && vb == kv::kExpNan;
+        // Exponent of the key's values over the item's reference.
+        float e1 = dead || v_nan ? 0.f : (float)(vb - kv::kExpBias - ref);
 
         ok = ok && wait.warp(&sh.s_full, n & 1);
         ptx::tc_fence_after();
@@ -1089,7 +1340,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
 
         // Does a row rise above its maximum by more than kRise? Then the
         // largest s + e of each row over the tile is its new one.
-        const bool rise = any_of(t == s.t0 || high + vexp > kRise || !ok);
+        const bool up = high + e1 > kRise || fabsf(e1) > kWide;
+        const bool rise = any_of(first || up || !ok);
         // P's buffer is free: the product that read it two tiles ago was
         // issued before these scores, whose completion covers it. With one
         // buffer the product of the tile before has to be waited for.
@@ -1097,13 +1349,21 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         if (rise) {
           // A row of zeros has the exponent of 1 whatever its neighbours have. It
           // adds nothing under any exponent, and as one of 1 it would be the
-          // maximum of keys whose values are small, whose terms then vanish: the
-          // least one. Looked at only where it could set a maximum.
-          const bool look = vb == kv::kExpBias && !dead && (t == s.t0 || high + vexp > kRise);
+          // maximum of keys whose values are small, whose terms then vanish.
+          // Looked at only where it could set a maximum.
+          bool zero = false;
+          const bool look = (first || up) && !dead && vb == kv::kExpBias;
           if (__any_sync(0xffffffffu, look)) {
             const int st = (2 * n + 1) % NS;
             ok = ok && wait.warp(&sh.kv_full[st], ((2 * n + 1) / NS) & 1);
-            if (look && zero_row<D>(smem + st * C::kSlotBytes, tid)) vexp = (float)kv::kMinExp;
+            if (look) zero = zero_row<D>(smem + st * C::kSlotBytes, tid);
+          }
+          if (first) {  // (ref is 0: e1 is the exponent)
+            const float e_w = warp_max(dead || v_nan || zero ? -INFINITY : e1);
+            if (lane == 0) reinterpret_cast<float*>(&g.e_max)[wq] = e_w;
+            if (zero) e1 = fmaxf(e_w, (float)kLeastRef) - kWide;
+          } else if (zero) {
+            e1 = -kWide;
           }
           float top = -INFINITY;
 #pragma unroll
@@ -1111,8 +1371,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             if (r / C::kStep * C::kStep < used) {
               float d0, d1;
               ptx::unpack2(d2[r / 2], d0, d1);
-              d0 = warp_max(d0 + vexp);
-              d1 = warp_max(d1 + vexp);
+              d0 = warp_max(d0 + e1);
+              d1 = warp_max(d1 + e1);
               if (lane == r) top = d0;
               if (lane == r + 1) top = d1;
             }
@@ -1122,14 +1382,22 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             left = true;
             break;
           }
+          if (first) {
+            const float e_max = fmaxf(fmaxf(g.e_max.x, g.e_max.y), fmaxf(g.e_max.z, g.e_max.w));
+            ref = e_max == -INFINITY ? 0 : max((int)e_max, kLeastRef);
+          }
+          // Exponents that one reference does not serve; zeros whose score is
+          // so far above the others that they set a maximum.
+          if (!(zero || dead || v_nan) && fabsf((float)(vb - kv::kExpBias - ref)) > kWide) sh.again = 1;
+          if (zero && !first && high - kWide > kRise) sh.again = 1;
           float f_lane = 1.f;
           if (lane < RW) {
             const float4 v4 = g.top[lane];
-            const float v = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
+            const float v = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w)) - (first ? (float)ref : 0.f);
             float by = 0.f;
-            if (v > (t == s.t0 ? -INFINITY : kRise)) {
+            if (v > (first ? -INFINITY : kRise)) {
               by = v;
-              f_lane = t == s.t0 ? 0.f : ptx::ex2(-v);
+              f_lane = first ? 0.f : ptx::ex2(-v);
               m_lane += v;
             }
             g.step[lane] = -by;
@@ -1143,6 +1411,18 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
               d2[r / 2] = ptx::fadd2(d2[r / 2], by.x);
               d2[r / 2 + 1] = ptx::fadd2(d2[r / 2 + 1], by.y);
             }
+          }
+          if (first && __any_sync(0xffffffffu, zero)) {
+            float above = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < RW; r += 2) {
+              if (r / C::kStep * C::kStep < used) {
+                float d0, d1;
+                ptx::unpack2(d2[r / 2], d0, d1);
+                above = ptx::fmax3(above, d0, d1);
+              }
+            }
+            if (zero && above > kWide - 1.f) sh.again = 1;
           }
           if (t > s.t0) {
             // The sums so far, rescaled; O when the tile before is in it.
@@ -1176,11 +1456,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         }
         // p, its sum, and the key's row of P: the terms side by side. A key
         // that some rows do not see may have a NaN factor: their product with
-        // it is then not formed (kPick).
+        // it is then not formed (kPick). The factor, 8 * 2^e over the reference,
+        // is a power of two by its bits (of exponents near the reference; other
+        // items are computed again).
+        const float vf = dead ? 0.f : __int_as_float((vb - ref + kPShift) << 23);
         uint8_t* const p_tile = p_tiles + n % C::kPBufs * C::kPBytes;
         auto emit = [&](auto pick) {
           constexpr bool kPick = decltype(pick)::value;
-          const uint64_t vf2 = ptx::pack2(vf, vf);
+          const float f = kPick && v_nan ? __int_as_float(0x7fc00000) : vf;
+          const uint64_t vf2 = ptx::pack2(f, f);
 #pragma unroll
           for (int c = 0; c < RW; c += 8) {
             if (c < used) {
@@ -1208,7 +1492,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             }
           }
         };
-        if (!plain && __any_sync(0xffffffffu, vb == kv::kExpNan))
+        if (__any_sync(0xffffffffu, v_nan))
           emit(std::true_type());
         else
           emit(std::false_type());
@@ -1249,14 +1533,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         id_lane = rw.row_id[w * RW + lane];
         const float sum = sum_of(g.sum[lane]);
         const float top = sum == 0.f ? -INFINITY : m_lane;
-        inv_lane = sum == 0.f ? 0.f : __fdividef(1.f / kPScale, sum);
+        // 2^ref / 8, what P was taken over, by the sum
+        inv_lane = sum == 0.f ? 0.f : __fdividef(__int_as_float((127 + ref - kPShift) << 23), sum);
         if (wq == 0) {
           if (!whole)
             a.part_ml[(long long)part * C::kRows + w * RW + lane] = make_float2(top, sum);
           else if (!a.own_rows)
             a.full_ml[id_lane] = make_float2(top, sum);
           else if (a.lse)
-            a.lse[id_lane] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+            a.lse[id_lane] = sum == 0.f ? -INFINITY : ln_of(top, sum);
         }
       }
       // (Should this wait give up, the next barrier ends the block.)
@@ -1282,15 +1567,16 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
 #pragma unroll
             for (int q = NT - 2; q >= 0; --q)
               v = fmaf(v, 1.f / kTerm, __uint_as_float(raw[q * 8 + e]));
+            v *= inv;
             if (r < used && (D == 128 || (r & 1) == tid / 64)) {
               if (!whole)
                 a.part_o[to + d] = v;
               else if (!a.own_rows)
                 a.full_o[to + d] = v;
               else if (kBf16)
-                reinterpret_cast<__nv_bfloat16*>(a.o)[to + d] = __float2bfloat16(v * inv);
+                reinterpret_cast<__nv_bfloat16*>(a.o)[to + d] = __float2bfloat16(v);
               else
-                reinterpret_cast<__half*>(a.o)[to + d] = __float2half(v * inv);
+                reinterpret_cast<__half*>(a.o)[to + d] = __float2half(v);
             }
           }
         }
@@ -1300,11 +1586,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       if (lane == 0) ptx::mbar_arrive(&sh.q_free[k & 1]);
       if (C::kHelperQ ? last : !walk.next(a, C::kItemCost, s)) break;
     }
+    end_sync();  // nothing is under way any more: the ring is free
+    if (sh.again && !sh.abort) share_again<C, kBf16>(a, sh.start, reinterpret_cast<float*>(smem));
   }
 
-  __syncwarp();
-  ptx::tc_fence_before();
-  __syncthreads();
   if (warp == C::kMmaWarp) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(sh.tmem, C::kTmemCols);
@@ -1315,10 +1600,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
 }
 
 // --------------------------------------------------------------------- joining
-// Sum of parts of one row, spread over a warp: lane holds D / 32 values.
+// Sum of parts of one row, spread over a warp: lane holds D / 32 values. A part
+// is its result o, the maximum m that its weights are relative to and their sum
+// l = 2^k x; it weighs 2^m l, and the joined row's m is the largest m + k. Results
+// are at most as large as values are: kLess keeps the sum of up to a thousand of
+// them, each weighing less than 2, inside fp32.
 template <int D>
 struct RowSum {
   static constexpr int V = D / 32;
+  static constexpr float kLess = 1.f / 2048;
   float m = -INFINITY, l = 0.f, o[V];
   __device__ __forceinline__ RowSum() {
 #pragma unroll
@@ -1345,12 +1635,15 @@ struct RowSum {
       const int here = min(32, n - i0);
       float2 ml = make_float2(-INFINITY, 0.f);
       if (lane < here) ml = __ldcg(pml + at(i0 + lane));
-      const float top = fmaxf(m, warp_max(ml.x));
+      const int k = log2_below(ml.y);
+      const float lead = ml.x + (float)k;
+      const float top = fmaxf(m, warp_max(lead));
       const float use = top == -INFINITY ? 0.f : top;
-      const float keep = ptx::ex2(m - use), w = ptx::ex2(ml.x - use);
-      float sum = w * ml.y;
+      const float keep = ptx::ex2(m - use);
+      float w = ptx::ex2(lead - use) * over_log2(ml.y, k), sum = w;
+      w *= kLess;
 #pragma unroll
-      for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+      for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
       l = l * keep + sum;
 #pragma unroll
       for (int e = 0; e < V; ++e) o[e] *= keep;
@@ -1375,7 +1668,7 @@ struct RowSum {
   template <bool kBf16>
   __device__ __forceinline__ void store(const Args& a, int b, int h, int i) const {
     const int lane = threadIdx.x % 32;
-    const float inv = l == 0.f ? 0.f : 1.f / (kPScale * l);
+    const float inv = l == 0.f ? 0.f : 1.f / (kLess * l);
     uint32_t w[V / 2];
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
@@ -1393,7 +1686,7 @@ struct RowSum {
       *reinterpret_cast<uint32_t*>(dst) = w[0];
     if (a.lse && lane == 0)
       a.lse[((long long)b * a.heads + h) * a.seqlen_q + i] =
-          l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          l == 0.f ? -INFINITY : ln_of(m, l);
   }
 };
 

@@ -39,9 +39,8 @@ struct CacheView {
 
 constexpr int kExpNan = 255;   // byte of a row that held an infinity or a NaN
 constexpr int kExpBias = 127;
-// Least exponent of a written row. Attention scales its probabilities by
-// 2^-e in fp32 (see fa8_decode.cu); 2^63 leaves its sums room for 2^63 keys.
-// Values below 2^-73, half the least subnormal code, become zero.
+// Least exponent of a written row: values below 2^-73, half the least subnormal
+// code, become zero. (Attention takes any: see kWide in fa8_decode.cu.)
 constexpr int kMinExp = -63;
 
 __device__ __forceinline__ float exp_factor(int byte) {

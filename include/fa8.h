@@ -368,6 +368,14 @@ int fa8_kv_read(const fa8_kv_copy_params* p, void* stream);
  * fp32 [batch][heads][seqlen_q], natural log, contiguous. Queries that see no
  * key give o = 0 and lse = -inf.
  *
+ * Exponent bytes may be any: sums and maxima are kept so that neither very large
+ * or small rows of V nor both beside each other leave the range of fp32 (rows of
+ * one sequence and head whose exponents differ by more than 24 take longer).
+ * Weights p = exp(s) are rounded to 11 (fp16) or 8 (bf16) bits, with a floor of
+ * 2^-21 or 2^-17 of the query's largest p_j * 2^e_j; one under 2^-126 of the
+ * query's largest may count as zero. A result beyond the type's range is
+ * infinite.
+ *
  * prefix_len > 0: the first prefix_len tokens of all sequences are the same
  * (the caller vouches for it). Whole pages of them are taken from row 0 of the
  * table alone, and all the batch's queries meet the prefix together where that

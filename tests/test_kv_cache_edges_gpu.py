@@ -1,5 +1,6 @@
 """GPU checks of the cache's attention where it can go wrong: calls whose waits run
-out beside calls of another stream; value rows of zeros.
+out beside calls of another stream; value rows of zeros, and of very different and
+very large or small values.
 
 Tolerances, with u = eps / 2 of q's type (2^-11 fp16, 2^-8 bf16), p the weights, w
 their sum, c_j the codes and 2^e_j the factor of value row j:
@@ -9,7 +10,11 @@ their sum, c_j the codes and 2^e_j the factor of value row j:
 * scores: fp32 sums of D products, each addition off by 2^-22 of the largest partial
   sum B, and q's elements by half the least step of the last term: ds = D 2^-22 B +
   2^-21 (bf16) or 2^-25 (fp16) of the row's largest |q| times the largest scale *
-  sum |k| of a key. It moves the quotient by 2 ds A. exp2 and sums: 2^-20 A;
+  sum |k| of a key. It moves the quotient by 2 ds A. exp2 and sums: 2^-20 A; where
+  exponents of values differ by E, weights are exponentials of numbers up to E + 8
+  that were rounded twice: 2^-23 E A;
+* results of parts are joined by their weights, and fp32 holds none under 2^-126
+  of the row's largest (rounded up to a power of two): 2^-125 sum |v_j|;
 * small p meet a floor, 2^-17 or 2^-21 of the row's largest p_j 2^e_j over rows j
   that are not zero, for every key: that times sum_j |c_j| / w.
 lse: ds + 2^-20 (1 + |lse|). A result beyond the type's largest is infinite.
@@ -73,7 +78,11 @@ def assert_near(got, q, cache, table, lens, scale=None):
             lead = torch.where(solid, s / math.log(2) + e[:, :m], -math.inf).amax(-1)
             lead = torch.exp2(lead - torch.logsumexp(s, -1) / math.log(2))
             floor = lead[:, None] * c[:, :m].abs().sum(1) * 2.0 ** (-21 if fp16 else -17)
-            tol = (u * want.abs()).clamp(min=least) + (u + 2 * ds[:, None] + 2.0 ** -20) * A + floor
+            E = (torch.where(solid, e[:, :m], -math.inf).amax(-1)
+                 - torch.where(solid, e[:, :m], math.inf).amin(-1)).clamp(min=0).unsqueeze(-1)
+            tol = ((u * want.abs()).clamp(min=least)
+                   + (u + 2 * ds[:, None] + 2.0 ** -20 + 2.0 ** -23 * E) * A + floor
+                   + 2.0 ** -125 * v[:, :m].abs().sum(1))
             err = (out[b, :, i].double() - want).abs()
             far = want.abs() > top  # may round to the largest or to infinity
             bad = (~(err <= tol)) & ~far
@@ -193,4 +202,124 @@ def test_shared_prefix_row_of_zeros(fa8, size, dtype):
     before = fa8.launch_count()
     got = fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix, return_lse=True)
     assert fa8.launch_count() - before == 3  # the prefix has a launch of its own
+    assert_near(got, q, cache, table, lens)
+
+
+def resized(cache, size, name="v"):
+    """The cache with its V (or K) rows multiplied by `size` (pages, heads, slots), float64."""
+    x = getattr(cache, name).double() * ref.factor(getattr(cache, name + "_exp")).unsqueeze(-1)
+    values, byte = ref.quantise(x * size.unsqueeze(-1))
+    return cache._replace(**{name: values.float().to(E4M3), name + "_exp": byte})
+
+
+SIZES = {  # powers of two that value rows (of about 1) are multiplied by, by position
+    "largest": lambda pos, rnd: 110 + 14 * rnd,
+    "least": lambda pos, rnd: -60 + 4 * rnd,
+    "any": lambda pos, rnd: -64 + 188 * rnd,
+    "growing": lambda pos, rnd: -60 + 184 * pos,
+    "shrinking": lambda pos, rnd: 124 - 184 * pos,
+    "few large": lambda pos, rnd: torch.where(rnd > 0.99, 120.0, 0.0),
+    "few small": lambda pos, rnd: torch.where(rnd > 0.99, -60.0, 20.0),
+    "late": lambda pos, rnd: torch.where(pos > 0.97, 123.0, -30.0),
+    "near": lambda pos, rnd: 48 * rnd,  # about as far apart as one reference serves
+}
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("sizes", list(SIZES))
+@pytest.mark.parametrize("D,H,Hkv,Sq,spread", [(128, 8, 2, 1, 1.0), (64, 4, 4, 3, 30.0),
+                                               (128, 32, 1, 2, 4.0), (128, 64, 1, 1, 60.0),
+                                               (64, 16, 2, 1, 1.0)])
+def test_decode_range_of_values(fa8, D, H, Hkv, Sq, spread, sizes, dtype):
+    """Values of any size beside each other; keys whose scores differ by up to hundreds."""
+    lens, ps = [700, 1300, 40, 129], 64
+    pages = pages_for(lens, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    table, seqlens = make_table(lens, ps, pages)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    power = torch.zeros(pages, Hkv, ps, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(lens):
+        for col in range(-(-n // ps)):
+            pos = (col * ps + torch.arange(ps, device="cuda").double()) / n
+            rnd = torch.rand(Hkv, ps, generator=g, device="cuda").double()
+            power[int(table[b, col])] = SIZES[sizes](pos.expand(Hkv, ps), rnd)
+    cache = resized(cache, torch.exp2(torch.floor(power)))
+    q = make_q(4, H, Sq, D, dtype, size=spread)
+    got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+    assert_near(got, q, cache, table, lens)
+    again = fa8.flash_attn_fp8_decode(q, cache, table, seqlens)
+    assert torch.equal(again.nan_to_num(7.0), got[0].nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("sizes", ["any", "late", "few large"])
+def test_shared_prefix_range_of_values(fa8, sizes, dtype):
+    D, H, Hkv, ps, prefix, B = 128, 32, 8, 16, 1040, 48
+    lens = [prefix + 1 + (7 * b) % 50 for b in range(B)]
+    table, seqlens, pages = shared_table(lens, prefix, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    rnd = torch.rand(pages, Hkv, ps, generator=g, device="cuda").double()
+    pos = torch.linspace(0, 1, pages * ps, device="cuda").double().view(pages, 1, ps)
+    cache = resized(cache, torch.exp2(torch.floor(SIZES[sizes](pos.expand(-1, Hkv, -1), rnd))))
+    same_prefix(cache, table, lens, prefix)
+    q = make_q(B, H, 1, D, dtype, size=3.0)
+    got = fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix, return_lse=True)
+    assert_near(got, q, cache, table, lens)
+
+
+def test_written_values_near_the_largest(fa8):
+    """bf16 rows of 1e30 to 3e38 through the write, beside ordinary ones."""
+    D, H, Hkv, ps, n = 128, 8, 2, 16, 300
+    g = torch.Generator(device="cuda").manual_seed(4)
+    cache = fa8.kv_cache_alloc(2 * 20, Hkv, ps, D)
+    table, seqlens = make_table([n, n], ps, 40)
+    x = torch.randn(2, 2, Hkv, n, D, generator=g, device="cuda").double()
+    power = 10 ** (30 + 8 * torch.rand(2, Hkv, n, 1, generator=g, device="cuda").double())
+    v = (x[1].clamp(-3, 3) * power).clamp(-3e38, 3e38)
+    v[1, :, ::2] = x[1][1, :, ::2]  # the second sequence: every other row an ordinary one
+    fa8.kv_cache_write(cache, x[0].bfloat16(), v.bfloat16(), table, seqlens)
+    q = make_q(2, H, 1, D, "bf16")
+    got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+    assert bool(torch.isfinite(got[1]).all())
+    assert_near(got, q, cache, table, [n, n])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("k_bytes,v_bytes,code", [
+    ((100, 130), (0, 3), 0x7e), ((100, 130), (250, 254), 0x38), ((100, 130), (0, 254), 0x38),
+    ((0, 2), (120, 130), 0x7e), ((0, 130), (110, 120), 0x7e)])
+def test_bytes_at_both_ends(fa8, k_bytes, v_bytes, code, dtype):
+    """A cache that a caller brings: any byte but 255, codes up to `code` for V."""
+    D, H, Hkv, ps = 64, 8, 2, 32
+    lens = [500, 33]
+    pages = pages_for(lens, ps)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    cache = make_cache(fa8, pages, Hkv, ps, D)
+    byte = lambda lo, hi: torch.randint(lo, hi + 1, (pages, Hkv, ps), generator=g,  # noqa: E731
+                                        device="cuda", dtype=torch.uint8)
+    codes = torch.randint(0, code + 1, cache.v.shape, generator=g, device="cuda", dtype=torch.uint8)
+    sign = torch.randint(0, 2, cache.v.shape, generator=g, device="cuda", dtype=torch.uint8) * 128
+    cache = cache._replace(v=(codes | sign).view(E4M3), k_exp=byte(*k_bytes), v_exp=byte(*v_bytes))
+    table, seqlens = make_table(lens, ps, pages)
+    q = make_q(2, H, 1, D, dtype, size=0.02)
+    got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+    assert_near(got, q, cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("above", [5.0, 25.0, 60.0, 300.0])
+@pytest.mark.parametrize("H,Hkv,zeros", [(8, 2, 1), (8, 2, 200), (64, 1, 130)])
+def test_decode_zeros_far_above(fa8, H, Hkv, zeros, above, dtype):
+    """Leading rows of zeros whose scores are far above the others', and far below."""
+    lens, ps, D = [640, 300], 16, 128
+    pages = pages_for(lens, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    table, seqlens = make_table(lens, ps, pages)
+    q = make_q(2, H, 1, D, dtype, size=1.0)
+    zero = torch.zeros(Hkv, D, dtype=torch.float64, device="cuda")
+    for b, sign in ((0, 1), (1, -1)):
+        for pos in range(zeros):
+            put_row(cache, table, ps, b, pos, toward(q[b], sign * above, Hkv), zero)
+    got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
     assert_near(got, q, cache, table, lens)
