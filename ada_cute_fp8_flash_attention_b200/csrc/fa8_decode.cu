@@ -23,9 +23,11 @@
 // e4m3 has 4 significant bits and a rounding is off by half a step, so two
 // terms hold 8 bits and three hold 11 or more: what bf16 and fp16 have. The
 // terms are columns of their own (N is 2 or 3 times the rows) and are added
-// up in fp32 with their weights. Q is held exactly (scaled by a power of two
-// per row so that its largest magnitude is in [128, 256)); P is rounded once
-// to 11 (fp16) or 8 (bf16) bits, as it would be for a 16-bit product.
+// up in fp32 with their weights. Q is scaled by a power of two per row so that
+// its largest magnitude is in [128, 256). The last term's least step is 2^-13
+// (bf16) or 2^-17 (fp16) there: elements from 2^-13 or 2^-14 of the largest up
+// are held exactly, smaller ones to 2^-21 or 2^-25 of it. P is rounded once to 11
+// (fp16) or 8 (bf16) bits, as it would be for a 16-bit product.
 //
 // Softmax in base 2 with one running maximum per row, m = max(s + e), e the
 // exponent of v_j over a reference, the largest of the item's first tile: then
@@ -614,7 +616,8 @@ __device__ __forceinline__ void prepare_rows(const Args& a, const Seg& s, Rows& 
       const uint32_t bits =
           kBf16 ? m << 16
                 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
-      // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 are as good as zero.
+      // 2^(7 - e) with 2^e <= max < 2^(e + 1); rows below 2^-100 (bf16) are held to
+      // 2^-121, as rows of 2^-100 are.
       const int e = m == 0 ? 7 : max((int)(bits >> 23) - 127, -100);
       if (cl == 0)
         rw.mul[first + r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23)

@@ -1,6 +1,6 @@
 """GPU checks of the cache's attention where it can go wrong: calls whose waits run
 out beside calls of another stream; value rows of zeros, and of very different and
-very large or small values.
+very large or small values; queries with one large element.
 
 Tolerances, with u = eps / 2 of q's type (2^-11 fp16, 2^-8 bf16), p the weights, w
 their sum, c_j the codes and 2^e_j the factor of value row j:
@@ -305,6 +305,20 @@ def test_bytes_at_both_ends(fa8, k_bytes, v_bytes, code, dtype):
     q = make_q(2, H, 1, D, dtype, size=0.02)
     got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
     assert_near(got, q, cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_query_with_one_large_element(fa8, dtype):
+    """The largest element meets zeros of K: the others are what the scores are made of."""
+    lens, D, H, Hkv = [600, 200], 128, 8, 2
+    cache = make_cache(fa8, pages_for(lens, 16), Hkv, 16, D, spread=0.3)
+    u8(cache.k)[..., 5] = 0
+    table, seqlens = make_table(lens, 16, pages_for(lens, 16))
+    for large in (64.0, 2048.0, 30000.0):
+        q = make_q(2, H, 1, D, dtype)
+        q[..., 5] = large
+        got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+        assert_near(got, q, cache, table, lens)
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
