@@ -239,13 +239,16 @@ def flash_attn_fp8_shared_prefix(q, cache, page_table, seqlens, prefix_len, soft
                                  return_lse=False, out=None, status=None):
     """``flash_attn_fp8_decode`` for a batch whose sequences begin with the same tokens.
 
-    The first ``prefix_len`` tokens (a host number, any value a table row can hold)
-    are taken from the pages of ``page_table``'s row 0 (the other rows' entries for
-    whole prefix pages are not read), and all the batch's queries meet them together;
-    a prefix too short for that to pay is met by each sequence for itself. The result
-    is that of ``flash_attn_fp8_decode`` up to the order of its sums, given that every
+    Of the first ``prefix_len`` tokens (a host number, any value a table row can hold)
+    those in whole pages, the first ``prefix_len // page_size`` columns, are taken from
+    ``page_table``'s row 0 for all sequences: row 0 lists these pages whatever
+    ``seqlens[0]`` is, and the other rows' entries for them are not read. Tokens behind
+    them, the page that the prefix ends in among them, come from each sequence's own
+    row. All the batch's queries meet the shared pages together; a prefix too short for
+    that to pay is met by each sequence for itself, from the same pages. The result is
+    that of ``flash_attn_fp8_decode`` up to the order of its sums, given that every
     row's first prefix_len tokens hold what row 0's hold. Sequences shorter than the
-    prefix see their own length of it.
+    prefix, the first one too, see their own length of it.
     """
     res = _C.flash_attn_fp8_decode(q, cache[0], cache[1], cache[2], cache[3], page_table, seqlens,
                                    int(prefix_len), softmax_scale, return_lse, out, status)

@@ -200,9 +200,8 @@ struct Args {
   long long q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
   int heads, group, seqlen_q;
   int prefix_mode;   // items are the shared prefix's (rows of all sequences)
-  int key0;          // first key of these items
-  int key_base;      // key0 rounded down to where a TMA box may start
-  int prefix_len;
+  int key0;          // first key of these items, the first of a page
+  int prefix_len;    // keys of the prefix's items
   int shared_pages;  // table columns that every sequence has in row 0
   int row_tiles;     // tiles of query rows per (sequence, K/V head)
   int box;           // keys of a TMA box: min(page_size, 128)
@@ -393,7 +392,7 @@ __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return len < 0 || len > a.c.max_len ? -1 : len;
 }
 __device__ __forceinline__ int tiles_of(const Args& a, int len) {
-  return len > a.key0 ? (len - a.key_base + kTileKeys - 1) / kTileKeys : 0;
+  return len > a.key0 ? (len - a.key0 + kTileKeys - 1) / kTileKeys : 0;
 }
 
 // A run of key tiles t0..t1-1 of one item (sequence b, K/V head, row tile).
@@ -690,8 +689,7 @@ __device__ __forceinline__ void share_again(const Args& a, Walk walk, float* scr
     const int used = min(C::kRows, rows - s.rt * C::kRows);
     const bool whole = s.t0 == 0 && s.t1 == s.nt;
     const int part = 2 * blockIdx.x + (k > 0 ? 1 : 0);
-    const int first = max(a.key0, a.key_base + s.t0 * kTileKeys);
-    const int last = min(s.len, a.key_base + s.t1 * kTileKeys);
+    const int first = a.key0 + s.t0 * kTileKeys, last = min(s.len, a.key0 + s.t1 * kTileKeys);
     const int* const table = c.table + (a.prefix_mode ? 0 : s.b) * c.table_stride;
 #pragma unroll 1
     for (int r0 = 0; r0 < used; r0 += R) {
@@ -1048,8 +1046,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         // Table entries of the item's next 32 pieces, one a lane: one load for 4
         // to 32 tiles, asked for a batch ahead.
         auto entries = [&](int piece) {
-          const int key = a.key_base + s.t0 * kTileKeys + (piece + lane) * a.box;
-          if (key >= min(s.len, a.key_base + s.t1 * kTileKeys)) return 0;
+          const int key = a.key0 + s.t0 * kTileKeys + (piece + lane) * a.box;
+          if (key >= min(s.len, a.key0 + s.t1 * kTileKeys)) return 0;
           const int col = page_of(a, key);
           return __ldg((col < a.shared_pages ? a.c.table : table) + col);
         };
@@ -1062,7 +1060,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             next = entries((t - s.t0) * pieces + 32);
           }
           const int page = __shfl_sync(0xffffffffu, cur, (piece + lane) & 31);
-          const int key0 = a.key_base + t * kTileKeys, key = key0 + lane * a.box;
+          const int key0 = a.key0 + t * kTileKeys, key = key0 + lane * a.box;
           const bool have = lane < pieces && key < s.len;
           // A page outside the cache: coordinates that read as zeros, exponents
           // that say NaN.
@@ -1275,10 +1273,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
       if (lane < RW) g.neg_m[lane] = 0.f;  // (every warp writes the same)
       __syncwarp();
       for (int t = s.t0; t < s.t1; ++t, ++n) {
-        const int first_key = a.key_base + t * kTileKeys, key = first_key + tid;
+        const int first_key = a.key0 + t * kTileKeys, key = first_key + tid;
         // Every key of the tile seen by every row? This one by any?
-        const bool plain = first_key >= a.key0 && first_key + kTileKeys <= all_see;
-        const bool dead = key < a.key0 || key >= s.len;
+        const bool plain = first_key + kTileKeys <= all_see, dead = key >= s.len;
         ok = ok && wait.warp(&sh.e_full[n % kExpTiles], (n / kExpTiles) & 1);
         const int kb = sh.exps[n % kExpTiles][0][tid], vb = sh.exps[n % kExpTiles][1][tid];
         const float kf = kv::exp_factor(kb);
@@ -1501,7 +1498,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
           emit(std::false_type());
         // Rows of V that are not this item's keys (the end of a page, a page
         // not brought in) may hold anything, NaN codes among them: zeros.
-        if (w == 0 && (first_key < a.key0 || first_key + kTileKeys > s.len)) {
+        if (w == 0 && first_key + kTileKeys > s.len) {
           const int st = (2 * n + 1) % NS;
           ok = ok && wait.warp(&sh.kv_full[st], ((2 * n + 1) / NS) & 1);
           if (dead) {
@@ -1857,6 +1854,12 @@ struct Layout {
 };
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
+// Keys that are taken from row 0 of the table for all sequences: those in whole
+// pages of the prefix, however they are met.
+int64_t shared_len(const fa8_decode_params* p) {
+  return p->prefix_len / p->cache.page_size * p->cache.page_size;
+}
+
 // Whether a prefix has a set of items of its own. Three launches in a row take
 // 16 us however little there is to do, two 10; met by every sequence for
 // itself (from the same pages, in L2) the prefix is more tiles to each block.
@@ -1865,11 +1868,10 @@ int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 // 2048 (14) 29 / 31, 64 behind 2048 (28) 40 / 51; 16 heads of D = 64, 444
 // blocks: 8 behind 1000 (2.3) 21 / 15, 48 behind 1024 (14) 30 / 39.
 bool prefix_apart(const fa8_decode_params* p) {
-  if (p->prefix_len == 0) return false;
   const int64_t rows = p->seqlen_q * (p->heads / p->cache.heads_kv);
   const Shape s = shape_for(rows);
   const int64_t tiles = (rows + s.tile_rows() - 1) / s.tile_rows() * p->cache.batch *
-                        p->cache.heads_kv * ((p->prefix_len + kTileKeys - 1) / kTileKeys);
+                        p->cache.heads_kv * ((shared_len(p) + kTileKeys - 1) / kTileKeys);
   return tiles > 10 * kSmCount * resident((int)p->cache.head_dim, s.rw, s.nwg);
 }
 
@@ -1979,11 +1981,11 @@ int run(const fa8_decode_params* p, Args a, char* ws, int dev, cudaStream_t stre
     const Layout l0 = layout_of(p, true, 0), l1 = layout_of(p, false, l0.end);
     Args b = a;
     b.prefix_mode = 1;
+    b.prefix_len = (int)shared_len(p);
     int st = run_set<D, kBf16>(p, b, l0, ws, dev, stream);
     if (st) return st;
     b = a;
-    b.key0 = a.prefix_len;
-    b.key_base = a.prefix_len / a.box * a.box;
+    b.key0 = (int)shared_len(p);
     b.early = 1;
     st = run_set<D, kBf16>(p, b, l1, ws, dev, stream);
     if (st) return st;
@@ -2029,6 +2031,7 @@ int64_t fa8_decode_workspace_size(const fa8_decode_params* p) {
   using namespace fa8::dec;
   if (!p || p->cache.batch < 0 || p->heads < 0 || p->seqlen_q < 0 || p->prefix_len < 0 ||
       (p->cache.head_dim != 64 && p->cache.head_dim != 128) || p->cache.heads_kv <= 0 ||
+      p->cache.page_size <= 0 || p->prefix_len > p->cache.max_pages * p->cache.page_size ||
       p->heads % p->cache.heads_kv != 0) {
     fa8_note_error(FA8_ERR_INVALID_ARG, "fa8_decode_workspace_size: sizes that fa8_decode refuses");
     return -1;
@@ -2061,7 +2064,6 @@ int fa8_decode(const fa8_decode_params* p, void* workspace, int64_t workspace_by
   a.heads = (int)p->heads;
   a.group = (int)(p->heads / p->cache.heads_kv);
   a.seqlen_q = (int)p->seqlen_q;
-  a.prefix_len = (int)p->prefix_len;
   const int page = (int)p->cache.page_size;
   a.box = std::min(page, kTileKeys);
   a.by_page = Divisor::of(page);

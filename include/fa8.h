@@ -378,10 +378,12 @@ int fa8_kv_read(const fa8_kv_copy_params* p, void* stream);
  * infinite.
  *
  * prefix_len > 0: the first prefix_len tokens of all sequences are the same
- * (the caller vouches for it). Whole pages of them are taken from row 0 of the
- * table alone, and all the batch's queries meet the prefix together where that
- * is faster than each sequence by itself (the rule goes by sizes). The result
- * is that of prefix_len = 0 up to the order of its sums.
+ * (the caller vouches for it). Those in whole pages, the first prefix_len /
+ * page_size columns, are taken from row 0 of the table alone, whatever seqlens[0]
+ * is; those behind them from each sequence's own row, up to its own length. All
+ * the batch's queries meet the shared pages together where that is faster than
+ * each sequence by itself (the rule goes by sizes). The result is that of
+ * prefix_len = 0 up to the order of its sums.
  *
  * The caller provides fa8_decode_workspace_size() bytes of device workspace,
  * 256-byte aligned; nothing in it is kept or expected between calls, and

@@ -337,3 +337,33 @@ def test_decode_zeros_far_above(fa8, H, Hkv, zeros, above, dtype):
             put_row(cache, table, ps, b, pos, toward(q[b], sign * above, Hkv), zero)
     got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
     assert_near(got, q, cache, table, lens)
+
+
+@pytest.mark.parametrize("B", [4, 64])
+@pytest.mark.parametrize("first", [0, 1, 700, 960, 975])
+def test_shared_prefix_behind_a_short_first_sequence(fa8, first, B):
+    """Whole prefix pages come from row 0 whatever its length, what is behind them from
+    each row: the same pages in a small batch and in a large one."""
+    D, H, Hkv, ps, prefix = 128, 32, 8, 64, 1000
+    lens = [prefix + 1 + (7 * b) % 90 for b in range(B)]
+    table, seqlens, pages = shared_table(lens, prefix, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    same_prefix(cache, table, lens, prefix)
+    col = prefix // ps
+    lens[0] = first
+    seqlens[0] = first
+    if first <= col * ps:
+        table[0, col] = -1  # the first sequence needs no page there
+    else:  # its own page holds its own tokens of the prefix, and then anything
+        page = int(table[0, col])
+        u8(cache.k)[page, :, first - col * ps:] = 0x7f
+        cache.v_exp[page, :, first - col * ps:] = 255
+    table[0, col + 1:] = -1
+    q = make_q(B, H, 1, D, "bf16")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    before = fa8.launch_count()
+    got = fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix, return_lse=True,
+                                           status=status)
+    assert fa8.launch_count() - before == (3 if B == 64 else 2)
+    assert int(status) == 0
+    assert_near(got, q, cache, table, lens)
