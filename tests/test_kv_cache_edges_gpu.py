@@ -367,3 +367,134 @@ def test_shared_prefix_behind_a_short_first_sequence(fa8, first, B):
     assert fa8.launch_count() - before == (3 if B == 64 else 2)
     assert int(status) == 0
     assert_near(got, q, cache, table, lens)
+
+
+def prefix_case(fa8, B, H, Hkv, Sq, D, prefix, ps, dtype, size=0.7):
+    """A batch for which the prefix has a launch of its own; one sequence ends inside it,
+    one is empty, one ends with it."""
+    lens = [prefix + Sq + (11 * b) % 140 for b in range(B)]
+    lens[1], lens[5], lens[7] = prefix - 3, 0, prefix
+    table, seqlens, pages = shared_table(lens, prefix, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    same_prefix(cache, table, lens, prefix)
+    return cache, table, seqlens, lens, make_q(B, H, Sq, D, dtype, size=size)
+
+
+def prefix_call(fa8, q, cache, table, seqlens, prefix, **kw):
+    before = fa8.launch_count()
+    got = fa8.flash_attn_fp8_shared_prefix(q, cache, table, seqlens, prefix, return_lse=True, **kw)
+    assert fa8.launch_count() - before == 3  # the prefix, what is behind it, the join
+    return got
+
+
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16"), (128, "fp16")])
+@pytest.mark.parametrize("ps,prefix", [(16, 1009), (32, 1000), (64, 1024), (128, 1300), (256, 1500),
+                                       (384, 1600), (1024, 1024)])
+def test_prefix_apart_pages(fa8, ps, prefix, D, dtype):
+    cache, table, seqlens, lens, q = prefix_case(fa8, 48, 32, 16, 1, D, prefix, ps, dtype)
+    got = prefix_call(fa8, q, cache, table, seqlens, prefix)
+    assert_near(got, q, cache, table, lens)
+    again = prefix_call(fa8, q, cache, table, seqlens, prefix)
+    assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+
+
+@pytest.mark.parametrize("B,H,Hkv,Sq,D", [(64, 64, 8, 1, 128), (32, 32, 8, 5, 64), (400, 8, 8, 1, 64),
+                                          (20, 16, 2, 33, 128)])
+def test_prefix_apart_row_shapes(fa8, B, H, Hkv, Sq, D):
+    prefix = 1500
+    cache, table, seqlens, lens, q = prefix_case(fa8, B, H, Hkv, Sq, D, prefix, 32, "bf16")
+    got = prefix_call(fa8, q, cache, table, seqlens, prefix)
+    assert_near(got, q, cache, table, lens)
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_prefix_apart_nan_rows(fa8, where):
+    """A NaN token inside the prefix reaches the queries that see it, one behind it its
+    own sequence's."""
+    prefix, Sq = 1100, 3
+    cache, table, seqlens, lens, q = prefix_case(fa8, 48, 32, 8, Sq, 128, prefix, 16, "fp16")
+    clean, _ = prefix_call(fa8, q, cache, table, seqlens, prefix)
+    exps = cache.k_exp if where == "k" else cache.v_exp
+    codes = u8(cache.k if where == "k" else cache.v)
+    lens[9] = seqlens[9] = prefix + 40
+    for b, pos, head in ((0, 1080, 2), (9, prefix + 38, 5)):  # the second: one of its queries is before it
+        page, slot = int(table[b, pos // 16]), pos % 16
+        exps[page, head, slot] = 255
+        codes[page, head, slot] = 0
+    out, lse = prefix_call(fa8, q, cache, table, seqlens, prefix)
+    want = torch.zeros(48, 32, Sq, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(lens):
+        for i in range(Sq):
+            want[b, 8:12, i] = n - Sq + i >= 1080
+    want[9, 20:24, 1:] = True
+    bad = out.isnan()
+    assert torch.equal(bad.all(-1), want) and torch.equal(bad.any(-1), want)
+    keep = ~want
+    keep[9] = False  # another length than before
+    assert torch.equal(out[keep], clean[keep])
+    assert not bool(lse[~want].isnan().any())
+
+
+def test_prefix_apart_bad_pages(fa8):
+    """Page ids outside the cache, inside the prefix and behind it; a refused length."""
+    prefix, ps = 1024, 16
+    cache, table, seqlens, lens, q = prefix_case(fa8, 48, 32, 8, 1, 128, prefix, ps, "bf16")
+    clean, _ = prefix_call(fa8, q, cache, table, seqlens, prefix)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    bad = table.clone()
+    bad[3, prefix // ps] = cache.k.shape[0]
+    bad[4, prefix // ps] = -(1 << 31)
+    out, lse = prefix_call(fa8, q, cache, bad, seqlens, prefix, status=status)
+    assert int(status) == 8
+    for b in range(48):
+        if b in (3, 4):
+            assert bool(out[b].isnan().all()) and bool(lse[b].isnan().all())
+        else:
+            assert torch.equal(out[b], clean[b])
+    bad = table.clone()
+    bad[0, 30] = 1 << 30  # of the prefix: all sequences but those that end before it
+    status.zero_()
+    out, _ = prefix_call(fa8, q, cache, bad, seqlens, prefix, status=status)
+    assert int(status) == 8
+    seen = torch.tensor(lens, device="cuda") > 30 * ps
+    assert torch.equal(out.isnan().all(-1).all(-1).all(-1), seen)
+    assert bool((out[~seen] == clean[~seen]).all())
+    status.zero_()
+    seqlens[2], seqlens[6] = -1, table.shape[1] * ps + 1
+    out = torch.full_like(q, 5.0)
+    prefix_call(fa8, q, cache, table, seqlens, prefix, out=out, status=status)
+    assert int(status) == 4 and bool((out[2] == 5).all()) and bool((out[6] == 5).all())
+    tol = 2 * torch.finfo(q.dtype).eps * (clean.abs() + 1)  # other shares of the work: other sums
+    keep = [b for b in range(48) if b not in (2, 6)]
+    assert bool(((out - clean).abs() <= tol)[keep].all())
+
+
+def test_prefix_apart_captured(fa8):
+    """The chain of three launches in a graph: replayed back to back, with other lengths,
+    on a side stream beside eager calls."""
+    prefix, ps = 1024, 16
+    cache, table, seqlens, lens, q = prefix_case(fa8, 48, 32, 8, 1, 128, prefix, ps, "bf16")
+    room = table.shape[1] * ps
+    table = table.clamp(min=0)  # every row full: the lengths change
+    prefix_call(fa8, q, cache, table, seqlens, prefix)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = prefix_call(fa8, q, cache, table, seqlens, prefix)
+    side = torch.cuda.Stream()
+    for lengths in (lens, [room - 7 * b % 50 for b in range(48)], [prefix] * 48, [0] * 48,
+                    [1 + 24 * b for b in range(48)]):
+        assert max(lengths) <= room
+        seqlens.copy_(torch.tensor(lengths))
+        want = prefix_call(fa8, q, cache, table, seqlens, prefix)
+        for t in got:
+            t.fill_(3.0)
+        torch.cuda.synchronize()
+        eager = []
+        with torch.cuda.stream(side):
+            for _ in range(10):
+                g.replay()
+        for _ in range(10):
+            eager.append(prefix_call(fa8, q, cache, table, seqlens, prefix))
+        torch.cuda.synchronize()
+        for o, l in [got] + eager:
+            assert torch.equal(o, want[0]) and torch.equal(l, want[1])
