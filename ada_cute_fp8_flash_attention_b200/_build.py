@@ -13,6 +13,7 @@ reference built its extension with ``-gencode arch=compute_89,code=sm_89``
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -54,6 +55,26 @@ def ext_path() -> Path:
     return PKG / f"{EXT_NAME}{suffix}"
 
 
+def check_decode_registers(log: str) -> int:
+    """Checks ptxas's register counts of the decode kernels; returns how many it saw.
+
+    The kernels move registers between their warps (setmaxnreg) and count on having
+    been given all that their launch bounds allow: 65536 / (blocks an SM * threads),
+    rounded down to 8. `log` is what nvcc prints under -Xptxas -v.
+    """
+    seen = 0
+    for m in re.finditer(r"decode_kernel\w*CfgILi(\d+)ELi\d+ELi(\d+)ELi(\d+)E.*?Used (\d+) registers",
+                         log, re.S):
+        dim, rows, groups, used = map(int, m.groups())
+        blocks = 1 if groups > 2 else 3 if dim == 64 and rows == 8 else 2
+        want = 65536 // (blocks * (groups * 128 + 128)) // 8 * 8
+        if used != want:
+            raise RuntimeError(f"decode_kernel (D {dim}, {groups} x {rows} rows) was given {used} "
+                               f"registers a thread, its register split needs {want}")
+        seen += 1
+    return seen
+
+
 def build_lib(force: bool = False, verbose: bool = False) -> Path:
     deps = [CSRC / s for s in CUDA_SOURCES + CUDA_HEADERS] + [INCLUDE / "fa8.h"]
     if not force and not _stale(LIB, deps):
@@ -66,6 +87,8 @@ def build_lib(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     if verbose:
         sys.stderr.write(res.stderr)
+    if not check_decode_registers(res.stdout + res.stderr):
+        raise RuntimeError("no register counts of the decode kernels in nvcc's output")
     os.replace(tmp, LIB)
     return LIB
 

@@ -1919,17 +1919,26 @@ int launch_set(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, int 
                cudaStream_t stream) {
   static std::once_flag flags[64];
   static cudaError_t errs[64];
+  static int regs[64];
   if (dev < 0 || dev >= 64) return fa8_note_error(FA8_ERR_INVALID_ARG, "device index out of range");
   auto kernel = decode_kernel<C, kBf16>;
   std::call_once(flags[dev], [&] {
     errs[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     cudaFuncAttributes at;
     if (errs[dev] == cudaSuccess) errs[dev] = cudaFuncGetAttributes(&at, kernel);
-    // The register split draws on what the block is launched with.
-    if (errs[dev] == cudaSuccess && at.numRegs != C::kRegsLaunch)
-      errs[dev] = cudaErrorInvalidKernelImage;
+    if (errs[dev] == cudaSuccess) regs[dev] = at.numRegs;
   });
   if (errs[dev] != cudaSuccess) return fa8_note_cuda_error(errs[dev], "decode kernel attributes");
+  // The register split draws on what the block is launched with: with less than
+  // its sum a warpgroup would wait for registers for ever. (The build checks it.)
+  if (C::NWG * C::kRegsSoft + C::kRegsHelp > (C::NWG + 1) * regs[dev]) {
+    char msg[160];
+    snprintf(msg, sizeof(msg),
+             "fa8_decode: this build's kernel has %d registers a thread, its split between the "
+             "warps needs %d: rebuild with the compiler and flags of _build.py",
+             regs[dev], C::kRegsLaunch);
+    return fa8_note_error(FA8_ERR_UNSUPPORTED, msg);
+  }
   const cudaError_t e = launch_early(kernel, dim3((unsigned)grid), C::kThreads, C::kSmem, stream,
                                      a.early != 0, tk, tv, a);
   return e == cudaSuccess ? FA8_OK : fa8_note_cuda_error(e, "decode kernel launch");
