@@ -93,6 +93,8 @@
 namespace fa8 {
 namespace dec {
 
+using kv::Divisor;
+
 constexpr int kTileKeys = 128;
 constexpr int kMostItemCost = 8;
 constexpr int kAgainBar = 6;           // named barrier of share_again
@@ -175,21 +177,6 @@ struct Cfg {
   static_assert(kSlots >= 4, "a K and a V tile in use and two on their way");
   static_assert(RW == 8 || RW == 16, "rows of a warpgroup");
   static_assert(kN <= 128 && kSlotBytes % 1024 == 0 && kPBytes % 1024 == 0, "tile alignment");
-};
-
-// x / d for 0 <= x < 2^31 by one multiplication.
-struct Divisor {
-  uint32_t mul, shift;
-  int d;
-  static Divisor of(int d) {
-    Divisor v{0, 0, d};
-    while ((1ll << v.shift) < d) ++v.shift;
-    v.mul = (uint32_t)((((1ull << v.shift) - d) << 32) / d + 1);
-    return v;
-  }
-  __device__ __forceinline__ int div(int x) const {
-    return (int)((__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
-  }
 };
 
 struct Args {

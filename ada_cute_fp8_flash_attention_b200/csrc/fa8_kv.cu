@@ -86,7 +86,7 @@ struct CopyArgs {
   int total;                // tokens of the call
   int tokens;               // per sequence, without cu
   int per_block;            // tokens of a block
-  uint32_t head_mul, head_shift;  // x / heads_kv = (mulhi(x, mul) + x) >> shift
+  Divisor by_heads;         // (heads_kv)
   long long k_sb, k_sh, k_ss, v_sb, v_sh, v_ss;
 };
 
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_row_kernel(const CopyArg
   constexpr int kLanes = D / 8;
   const int lane = threadIdx.x % kLanes;
   const int row = (blockIdx.x * kCopyThreads + threadIdx.x) / kLanes;
-  const int tok = (int)((__umulhi((uint32_t)row, a.head_mul) + (uint32_t)row) >> a.head_shift);
+  const int tok = a.by_heads.div(row);
   const int head = row - tok * a.c.heads_kv;
   const Place p = place_of(a, tok);
   const CacheView& c = a.c;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kCopyThreads, kWrite ? 8 : 1) kv_copy_kernel(c
 #pragma unroll
       for (int u = 0; u < kRowsInFlight; ++u) {
         const int r = r0 + u * kGroups;
-        tok[u] = (int)((__umulhi((uint32_t)r, a.head_mul) + (uint32_t)r) >> a.head_shift);
+        tok[u] = a.by_heads.div(r);
         head[u] = r - tok[u] * c.heads_kv;
         xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
         if (r >= rows || places[tok[u]].page < 0) {
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kCopyThreads, kWrite ? 8 : 1) kv_copy_kernel(c
 #pragma unroll
       for (int u = 0; u < kRowsInFlight; ++u) {
         const int r = r0 + u * kGroups;
-        tok[u] = (int)((__umulhi((uint32_t)r, a.head_mul) + (uint32_t)r) >> a.head_shift);
+        tok[u] = a.by_heads.div(r);
         head[u] = r - tok[u] * c.heads_kv;
         ck[u] = cv[u] = make_uint2(0, 0);
         bk[u] = bv[u] = kExpNan;
@@ -379,10 +379,8 @@ int copy(const fa8_kv_copy_params* p, void* stream) {
     return fa8_note_error(FA8_ERR_UNSUPPORTED, "cache copy: too many tokens");
   a.tokens = (int)p->tokens;
   a.total = (int)total;
-  const uint32_t heads = (uint32_t)p->cache.heads_kv;
-  a.head_shift = 0;
-  while ((1u << a.head_shift) < heads) ++a.head_shift;
-  a.head_mul = (uint32_t)((((1ull << a.head_shift) - heads) << 32) / heads + 1);
+  const int64_t heads = p->cache.heads_kv;
+  a.by_heads = Divisor::of((int)heads);
   a.k_sb = p->k_stride_b;
   a.k_sh = p->k_stride_h;
   a.k_ss = p->k_stride_s;

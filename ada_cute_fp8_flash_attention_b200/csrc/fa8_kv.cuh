@@ -22,6 +22,24 @@ void fa8_note_launch();
 namespace fa8 {
 namespace kv {
 
+// x / d for 0 <= x < 2^31 by one multiplication (the division by an invariant of
+// Granlund and Montgomery, PLDI 1994): with 2^shift the least power of two that is
+// not below d and mul = floor(2^32 (2^shift - d) / d) + 1, the quotient is
+// (floor(mul x / 2^32) + x) / 2^shift; x below 2^31 keeps that sum in 32 bits.
+struct Divisor {
+  uint32_t mul, shift;
+  int d;
+  static Divisor of(int d) {
+    Divisor v{0, 0, d};
+    while ((1ll << v.shift) < d) ++v.shift;
+    v.mul = (uint32_t)((((1ull << v.shift) - d) << 32) / d + 1);
+    return v;
+  }
+  __device__ __forceinline__ int div(int x) const {
+    return (int)((__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
+  }
+};
+
 struct CacheView {
   uint8_t* k;
   uint8_t* v;

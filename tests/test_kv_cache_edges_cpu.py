@@ -1,5 +1,8 @@
-"""CPU checks around the cache's attention: what the build verifies."""
+"""CPU checks around the cache's attention: what the build verifies, the division by
+an invariant."""
 from __future__ import annotations
+
+import random
 
 import pytest
 
@@ -22,3 +25,18 @@ def test_build_checks_the_register_split():
     for bad in (_log(126), good + _log(72, rows=16, groups=2), _log(88, dim=64)):
         with pytest.raises(RuntimeError, match="registers a thread"):
             _build.check_decode_registers(bad)
+
+
+def test_division_by_one_multiplication():
+    """The formula of fa8_kv.cuh's Divisor, over the whole range that it is used in."""
+    rng = random.Random(1)
+    for d in [*range(1, 200), 1023, 1024, 1025, 65535, 1 << 20, (1 << 30) + 7, (1 << 31) - 1]:
+        shift = (d - 1).bit_length()
+        mul = (((1 << shift) - d) << 32) // d + 1
+        assert mul < 1 << 32
+        last = (1 << 31) - 1
+        for x in [0, 1, d - 1, d, d + 1, 2 * d - 1, last, (last + 1) // d * d - 1,
+                  *(rng.randrange(1 << 31) for _ in range(50))]:
+            if 0 <= x <= last:
+                total = (mul * x >> 32) + x
+                assert total < 1 << 32 and total >> shift == x // d
