@@ -13,6 +13,7 @@
 // flash_attn_fp8_forward_ex adds: non-causal mode, an explicit scale,
 // V in BHSD layout, LSE output, e4m3 output, context-parallel offsets, the
 // P-split threshold and caller-provided output buffers.
+#include <limits>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -448,6 +449,12 @@ torch::Tensor device_i32(const torch::Tensor& t, const torch::Tensor& like, cons
   TORCH_CHECK(t.device().is_cpu() || t.device() == like.device(), name,
               " must be on the cache's device (or on the host)");
   TORCH_CHECK(at::isIntegralType(t.scalar_type(), false), name, " must hold integers");
+  // What does not fit 32 bits becomes their largest or least value, which the
+  // kernels refuse, not its low half, which may be a page or a length.
+  if (t.element_size() > 4)
+    return t.to(at::kLong)
+        .clamp(std::numeric_limits<int>::min(), std::numeric_limits<int>::max())
+        .to(like.device(), at::kInt);
   return t.to(like.device(), at::kInt);
 }
 

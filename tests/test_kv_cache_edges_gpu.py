@@ -498,3 +498,34 @@ def test_prefix_apart_captured(fa8):
         torch.cuda.synchronize()
         for o, l in [got] + eager:
             assert torch.equal(o, want[0]) and torch.equal(l, want[1])
+
+
+@pytest.mark.parametrize("host", [False, True])
+def test_wide_integers_are_not_cut(fa8, host):
+    """64-bit page ids and lengths beyond 32 bits are refused like any other."""
+    D, Hkv, ps = 64, 2, 16
+    cache = make_cache(fa8, 8, Hkv, ps, D)
+    table = torch.arange(8, dtype=torch.int64).view(2, 4)
+    lens = torch.tensor([50, 20])
+    place = (lambda t: t) if host else (lambda t: t.cuda())  # noqa: E731
+    q = make_q(2, 4, 1, D, "fp16")
+    want = fa8.flash_attn_fp8_decode(q, cache, place(table), place(lens))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for far in (1 << 32, -(1 << 32), 1 << 62):
+        bad = table.clone()
+        bad[0, 1] += far
+        status.zero_()
+        out = fa8.flash_attn_fp8_decode(q, cache, place(bad), place(lens), status=status)
+        assert int(status) == 8 and bool(out[0].isnan().all()) and torch.equal(out[1], want[1])
+        status.zero_()
+        out = torch.full_like(q, 5.0)
+        fa8.flash_attn_fp8_decode(q, cache, place(table), place(lens + torch.tensor([far, 0])),
+                                  out=out, status=status)
+        assert int(status) == 4 and bool((out[0] == 5).all())
+        assert float((out[1] - want[1]).abs().max()) <= 2 * torch.finfo(q.dtype).eps * (
+            1 + float(want[1].abs().max()))
+        x = torch.randn(2, Hkv, 1, D, device="cuda").half()
+        before = u8(cache.k).clone()
+        status.zero_()
+        fa8.kv_cache_write(cache, x, x, place(table), place(lens + far), status=status)
+        assert int(status) == 4 and torch.equal(u8(cache.k), before)
