@@ -529,3 +529,73 @@ def test_wide_integers_are_not_cut(fa8, host):
         status.zero_()
         fa8.kv_cache_write(cache, x, x, place(table), place(lens + far), status=status)
         assert int(status) == 4 and torch.equal(u8(cache.k), before)
+
+
+def c_copy(cache, table, seqlens, k, v, cu=None, status=None):
+    """The C ABI's parameters of a copy of packed (with cu) or dense contiguous rows."""
+    from ada_cute_fp8_flash_attention_b200 import c_abi
+    pages, heads_kv, page_size, D = cache.k.shape
+    p = c_abi.kv_copy_params(pages, heads_kv, page_size, D, seqlens.numel(), table.shape[1])
+    c = p.cache
+    c.k, c.v = cache.k.data_ptr(), cache.v.data_ptr()
+    c.k_exp, c.v_exp = cache.k_exp.data_ptr(), cache.v_exp.data_ptr()
+    c.page_table, c.seqlens = table.data_ptr(), seqlens.data_ptr()
+    c.status = status.data_ptr() if status is not None else None
+    p.k, p.v = k.data_ptr(), v.data_ptr()
+    p.dtype = c_abi.FA8_DT_BF16 if k.dtype == torch.bfloat16 else c_abi.FA8_DT_F16
+    if cu is not None:
+        p.cu_seqlens, p.tokens = cu.data_ptr(), k.shape[0]
+        p.k_stride_s, p.k_stride_h = k.stride(0), k.stride(1)
+        p.v_stride_s, p.v_stride_h = v.stride(0), v.stride(1)
+    else:
+        p.tokens = k.shape[2]
+        p.k_stride_b, p.k_stride_h, p.k_stride_s = k.stride()[:3]
+        p.v_stride_b, p.v_stride_h, p.v_stride_s = v.stride()[:3]
+    return p
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,heads_kv,n", [(64, 3, 5), (128, 8, 300)])
+def test_c_abi_write_read_decode(fa8, D, heads_kv, n, dtype):
+    """The C entry points on a side stream give what the torch ones do, packed and dense."""
+    from ada_cute_fp8_flash_attention_b200 import c_abi
+    B, ps = 3, 32
+    lens = [n + 40, n, n + 7]
+    pages = pages_for(lens, ps)
+    table, seqlens = make_table(lens, ps, pages)
+    x = torch.randn(2, B, heads_kv, n, D, device="cuda").to(dtype)
+    packed = [t.transpose(1, 2).reshape(B * n, heads_kv, D).contiguous() for t in x]
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda") * n
+    want = make_cache(fa8, pages, heads_kv, ps, D)
+    dense, rows = (type(want)(*(u8(t).clone().view(t.dtype) for t in want)) for _ in range(2))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    fa8.kv_cache_write(want, x[0], x[1], table, seqlens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    c_abi.check(c_abi.kv_write(c_copy(dense, table, seqlens, x[0], x[1], status=status),
+                               side.cuda_stream))
+    c_abi.check(c_abi.kv_write(c_copy(rows, table, seqlens, *packed, cu=cu, status=status),
+                               side.cuda_stream))
+    back = [torch.zeros_like(t) for t in packed]
+    c_abi.check(c_abi.kv_read(c_copy(rows, table, seqlens, *back, cu=cu, status=status),
+                              side.cuda_stream))
+    back4 = [torch.zeros_like(t) for t in x]
+    c_abi.check(c_abi.kv_read(c_copy(dense, table, seqlens, *back4, status=status),
+                              side.cuda_stream))
+    q = make_q(B, 2 * heads_kv, 1, D, "bf16" if dtype == torch.bfloat16 else "fp16")
+    side.wait_stream(torch.cuda.current_stream())
+    out, lse = torch.zeros_like(q), torch.zeros(q.shape[:3], device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    p, ws = c_decode(dense, table, seqlens, q, out, status, lse=lse)
+    c_abi.check(c_abi.decode(p, ws.data_ptr(), ws.numel(), side.cuda_stream))
+    side.synchronize()
+    assert int(status) == 0
+    for a, b, c in zip(want, dense, rows):
+        assert torch.equal(u8(a), u8(b)) and torch.equal(u8(a), u8(c))
+    name = "bf16" if dtype == torch.bfloat16 else "fp16"
+    k, v = fa8.kv_cache_read(want, table, seqlens, None, n, dtype=name)
+    assert torch.equal(back4[0], k) and torch.equal(back4[1], v)
+    k, v = fa8.kv_cache_read(want, table, seqlens, cu, B * n, dtype=name)
+    assert torch.equal(back[0], k) and torch.equal(back[1], v)
+    o, l = fa8.flash_attn_fp8_decode(q, want, table, seqlens, return_lse=True)
+    assert torch.equal(out, o) and torch.equal(lse, l)
