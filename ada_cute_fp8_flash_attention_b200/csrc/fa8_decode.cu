@@ -690,6 +690,9 @@ __device__ __forceinline__ void share_again(const Args& a, Walk walk, float* scr
           const unsigned short w = __ldg(reinterpret_cast<const unsigned short*>(a.q) +
                                          row.b * a.q_sb + row.h * a.q_sh + row.i * a.q_ss + i % D);
           x = kBf16 ? __uint_as_float((uint32_t)w << 16) : __half2float(__ushort_as_half(w));
+          // 2^20 less: D products of the largest bf16 with codes stay in fp32. A row
+          // with an infinity is NaN, as it is on the tensor cores.
+          x = fabsf(x) < INFINITY ? x * 0x1p-20f : __int_as_float(0x7fc00000);
         }
         q_s[i] = x;
       }
@@ -754,7 +757,7 @@ __device__ __forceinline__ void share_again(const Args& a, Walk walk, float* scr
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float sc = key < lim[r] ? y[r] * a.scale_log2 * kf : -INFINITY;
+          const float sc = key < lim[r] ? y[r] * kf * (a.scale_log2 * 0x1p20f) : -INFINITY;
           const float t = any && vb != kv::kExpNan ? sc + e : -INFINITY;
           const float m_new = fmaxf(ms[r], warp_max(sc)), e_new = fmaxf(me[r], warp_max(t));
           const float m_use = m_new == -INFINITY ? 0.f : m_new, e_use = e_new == -INFINITY ? 0.f : e_new;

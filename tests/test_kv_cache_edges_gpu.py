@@ -599,3 +599,32 @@ def test_c_abi_write_read_decode(fa8, D, heads_kv, n, dtype):
     assert torch.equal(back[0], k) and torch.equal(back[1], v)
     o, l = fa8.flash_attn_fp8_decode(q, want, table, seqlens, return_lse=True)
     assert torch.equal(out, o) and torch.equal(lse, l)
+
+
+@pytest.mark.parametrize("size,k_byte", [(1e36, 8), (1e37, 4), (1e-28, 214), (1.0, 127)])
+def test_extreme_queries_over_values_of_any_size(fa8, size, k_byte):
+    """bf16 queries at both ends of the type over keys at the other end: the scores are
+    ordinary, whichever way an item is computed; a query with an infinity is NaN."""
+    D, H, Hkv, ps = 128, 8, 2, 32
+    lens = [300, 45]
+    pages = pages_for(lens, ps)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.0)
+    codes = torch.randint(0x20, 0x39, cache.k.shape, generator=g, device="cuda", dtype=torch.uint8)
+    sign = torch.randint(0, 2, cache.k.shape, generator=g, device="cuda", dtype=torch.uint8) * 128
+    cache = cache._replace(k=(codes | sign).view(E4M3), k_exp=torch.full_like(cache.k_exp, k_byte))
+    table, seqlens = make_table(lens, ps, pages)
+    for apart in (False, True):
+        if apart:  # exponents of V far apart
+            cache.v_exp.copy_(torch.randint(60, 200, cache.v_exp.shape, generator=g, device="cuda",
+                                            dtype=torch.uint8))
+        q = (size * make_q(2, H, 1, D, "bf16", size=1.0).float()).bfloat16()
+        got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+        assert_near(got, q, cache, table, lens)
+        q[0, 1, 0, :] = math.inf
+        q[1, 2, 0, 7] = -math.inf
+        out, lse = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+        want = torch.zeros(2, H, 1, dtype=torch.bool, device="cuda")
+        want[0, 1] = want[1, 2] = True
+        assert torch.equal(out.isnan().all(-1), want) and torch.equal(lse.isnan(), want)
+        assert torch.equal(out[~want], got[0][~want])
