@@ -149,9 +149,9 @@ class KVCacheFP8(NamedTuple):
     unit last stride, the others multiples of 16. The row of a token and head has the values
     ``code * 2**(exp - 127)``; 255 marks a row that held an infinity or a NaN and
     reads as NaN. Codes are finite (``kv_cache_write`` stores no others); any other byte
-    may be given, and rows of any size stand beside each other (attention takes longer
-    where the exponents of one head's V differ by more than 24). page_size is 16, 32, 64
-    or a multiple of 128, D 64 or 128.
+    may be given, and rows of any size stand beside each other (attention over V rows
+    with bytes outside 80..160 takes several times as long). page_size is 16, 32, 64 or a
+    multiple of 128, D 64 or 128.
     """
     k: Any
     v: Any

@@ -30,7 +30,7 @@
 // (fp16) or 8 (bf16) bits, as it would be for a 16-bit product.
 //
 // Softmax in base 2 with one running maximum per row, m = max(s + e), e the
-// exponent of v_j over a reference, the largest of the item's first tile: then
+// exponent of v_j over kRef, that of rows of unit normal values: then
 // p = 2^(s - m) enters the sum, and what goes to the product is 8 * 2^e * p <= 8
 // whatever the exponents are (times 2^5, the rise of a maximum that is let be:
 // nothing is looked at row by row, exchanged or rescaled before one rises
@@ -39,11 +39,13 @@
 // p. The sum is kept per thread, over its own keys, in fp32, and joined at the
 // end of a row's keys.
 //
-// p is as far from 1 as e is from 0. Within 2^24 the sum keeps its digits. Where
-// a key's exponent is further away, or a row of zeros (whose exponent says
-// nothing) has a score so high that it would set the maximum, the block computes
-// its share once more in fp32 when it is done (share_again): values of any size
-// beside each other are right, at a price that others do not pay.
+// The largest p is as far from 1 as e is from 0: within 2^40 the sum has room
+// and keeps its digits. Where a key's exponent is further away (rows of V below
+// 1e-12 or above 1e12), or a row of zeros (whose exponent says nothing) has a
+// score so high that it would set the maximum, the block computes its share once
+// more in fp32 when it is done (share_again): values of any size beside each
+// other are right, at a price that others do not pay. A reference of the item's
+// own, its first tile's largest exponent, cost every call 2 to 3 % more.
 //
 // A block: one or more softmax warpgroups (8 or 16 rows each), a warp that
 // brings tiles, a thread that issues products, two warps that prepare the next
@@ -101,8 +103,8 @@ constexpr int kAgainBar = 6;           // named barrier of share_again
 constexpr int kMostWarps = 16;         // that prepare Q, or of the softmax
 constexpr float kRise = 5.f;           // log2 of the rise of a maximum that is let be
 constexpr int kPShift = 3;             // 8 p 2^e <= 2^(3 + kRise) < 448
-constexpr float kWide = 24.f;          // how far exponents of V may be from the item's reference
-constexpr int kLeastRef = -100;        // least reference exponent
+constexpr int kRef = -7;               // exponents of V are taken over: that of unit normal rows
+constexpr float kWide = 40.f;          // how far from it they may be
 constexpr float kTerm = 16.f;          // weight of a term over the next
 constexpr long long kTimeout = 4000000000LL;
 constexpr int kWaitHintNs = 20000;
@@ -155,7 +157,7 @@ struct Cfg {
   static constexpr int kCtas = resident(D, RW, NWG);
   // 227 KB a block, 228 KB an SM of which each block takes 1 KB and its
   // static variables; 1 KB to align.
-  static constexpr int kStatic = 2736 + 80 * kRows + 16 * NWG;
+  static constexpr int kStatic = 2736 + 80 * kRows;
   static constexpr int kBudget = (kCtas == 1 ? 227 : (228 - kCtas) / kCtas) * 1024 - kStatic - 1024;
   // P in two buffers where four tiles of the ring still fit beside them: the
   // next one is then written while the product of this one runs.
@@ -467,7 +469,7 @@ struct __align__(16) Shared {
   uint64_t drain;
   uint32_t tmem;
   int abort;
-  int again;                 // an item's exponents of V are too far apart
+  int again;                 // kRef does not serve an exponent of V
   Walk start;                // where the block's share begins
   struct __align__(16) Rows {  // of an item; read four at a time
     float mul[C::kRows];     // scale * log2(e) * the power of two of the row of Q
@@ -483,7 +485,6 @@ struct __align__(16) Shared {
     float step[C::RW];       // and what the last rise added to that
     float4 sum[C::RW];       // the four warps' sums of a row
     float4 top[C::RW];       // and maxima of a tile
-    float4 e_max;            // the four warps' largest exponents of V in a first tile
   } g[C::NWG];
   static_assert(sizeof(Rows) % 16 == 0 && sizeof(Group) % 16 == 0, "read four at a time");
   static_assert(C::kSlots / 2 + 2 <= kExpTiles,
@@ -651,12 +652,12 @@ __device__ __forceinline__ void floats_of(uint32_t w, float (&x)[4]) {
 }
 
 // A block's share once more, by its softmax warps, in fp32 and straight from the
-// cache: for items whose values are so different in size that one reference does
-// not serve them (kWide). Four rows at a time; a warp takes every W-th run of 32
+// cache: for values so large or small that kRef does not serve them, or so far
+// apart. Four rows at a time; a warp takes every W-th run of 32
 // keys, a lane a key for the scores and D / 32 columns for the values. The
 // maximum of s is the weights' reference, that of s + e the sum of values', so
 // neither leaves the range of fp32. A call whose every share is computed again
-// takes six to eight times as long (64 sequences of up to 16384 keys 1190 us), 15
+// takes six to eight times as long (64 sequences of up to 16384 keys 1170 us), 15
 // times behind a shared prefix. Kept apart from the loop over tiles: as a branch
 // of it, with a second exponential for P, it cost every call 10 to 17 %.
 template <class C, bool kBf16>
@@ -1256,10 +1257,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
 #pragma unroll
       for (int r = 0; r < RW / 2; ++r) l2[r] = 0;
       // Running maximum of row `lane`. A row that sees any of this block's keys
-      // of the item sees some of the first tile: that one sets it, and the
-      // reference that exponents of V are taken over, its largest.
+      // of the item sees some of the first tile: that one sets it.
       float m_lane = 0.f;
-      int ref = 0;
       if (lane < RW) g.neg_m[lane] = 0.f;  // (every warp writes the same)
       __syncwarp();
       for (int t = s.t0; t < s.t1; ++t, ++n) {
@@ -1270,8 +1269,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         const int kb = sh.exps[n % kExpTiles][0][tid], vb = sh.exps[n % kExpTiles][1][tid];
         const float kf = kv::exp_factor(kb);
         const bool first = t == s.t0, v_nan = !dead && vb == kv::kExpNan;
-        // Exponent of the key's values over the item's reference.
-        float e1 = dead || v_nan ? 0.f : (float)(vb - kv::kExpBias - ref);
+        float e1 = v_nan ? 0.f : (float)(vb - (kv::kExpBias + kRef));  // over kRef
 
         ok = ok && wait.warp(&sh.s_full, n & 1);
         ptx::tc_fence_after();
@@ -1330,8 +1328,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
 
         // Does a row rise above its maximum by more than kRise? Then the
         // largest s + e of each row over the tile is its new one.
-        const bool up = high + e1 > kRise || fabsf(e1) > kWide;
+        const bool up = high + e1 > kRise;
         const bool rise = any_of(first || up || !ok);
+        // An exponent that the reference does not serve.
+        if (!dead && fabsf(e1) > kWide) sh.again = 1;
         // P's buffer is free: the product that read it two tiles ago was
         // issued before these scores, whose completion covers it. With one
         // buffer the product of the tile before has to be waited for.
@@ -1348,13 +1348,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             ok = ok && wait.warp(&sh.kv_full[st], ((2 * n + 1) / NS) & 1);
             if (look) zero = zero_row<D>(smem + st * C::kSlotBytes, tid);
           }
-          if (first) {  // (ref is 0: e1 is the exponent)
-            const float e_w = warp_max(dead || v_nan || zero ? -INFINITY : e1);
-            if (lane == 0) reinterpret_cast<float*>(&g.e_max)[wq] = e_w;
-            if (zero) e1 = fmaxf(e_w, (float)kLeastRef) - kWide;
-          } else if (zero) {
-            e1 = -kWide;
-          }
+          // (Zeros so far above the others that they set a maximum all the same.)
+          if (zero) e1 = -kWide;
+          if (zero && !first && high - kWide > kRise) sh.again = 1;
           float top = -INFINITY;
 #pragma unroll
           for (int r = 0; r < RW; r += 2) {
@@ -1372,18 +1368,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             left = true;
             break;
           }
-          if (first) {
-            const float e_max = fmaxf(fmaxf(g.e_max.x, g.e_max.y), fmaxf(g.e_max.z, g.e_max.w));
-            ref = e_max == -INFINITY ? 0 : max((int)e_max, kLeastRef);
-          }
-          // Exponents that one reference does not serve; zeros whose score is
-          // so far above the others that they set a maximum.
-          if (!(zero || dead || v_nan) && fabsf((float)(vb - kv::kExpBias - ref)) > kWide) sh.again = 1;
-          if (zero && !first && high - kWide > kRise) sh.again = 1;
           float f_lane = 1.f;
           if (lane < RW) {
             const float4 v4 = g.top[lane];
-            const float v = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w)) - (first ? (float)ref : 0.f);
+            const float v = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
             float by = 0.f;
             if (v > (first ? -INFINITY : kRise)) {
               by = v;
@@ -1447,9 +1435,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         // p, its sum, and the key's row of P: the terms side by side. A key
         // that some rows do not see may have a NaN factor: their product with
         // it is then not formed (kPick). The factor, 8 * 2^e over the reference,
-        // is a power of two by its bits (of exponents near the reference; other
-        // items are computed again).
-        const float vf = dead ? 0.f : __int_as_float((vb - ref + kPShift) << 23);
+        // is a power of two by its bits (of exponents near the reference; shares
+        // with others are computed again).
+        const float vf = dead ? 0.f : __int_as_float((vb + (kPShift - kRef)) << 23);
         uint8_t* const p_tile = p_tiles + n % C::kPBufs * C::kPBytes;
         auto emit = [&](auto pick) {
           constexpr bool kPick = decltype(pick)::value;
@@ -1523,8 +1511,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         id_lane = rw.row_id[w * RW + lane];
         const float sum = sum_of(g.sum[lane]);
         const float top = sum == 0.f ? -INFINITY : m_lane;
-        // 2^ref / 8, what P was taken over, by the sum
-        inv_lane = sum == 0.f ? 0.f : __fdividef(__int_as_float((127 + ref - kPShift) << 23), sum);
+        // 2^kRef / 8, what P was taken over, by the sum
+        inv_lane = sum == 0.f ? 0.f : __fdividef(__int_as_float((127 + kRef - kPShift) << 23), sum);
         if (wq == 0) {
           if (!whole)
             a.part_ml[(long long)part * C::kRows + w * RW + lane] = make_float2(top, sum);

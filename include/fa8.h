@@ -369,8 +369,9 @@ int fa8_kv_read(const fa8_kv_copy_params* p, void* stream);
  * key give o = 0 and lse = -inf.
  *
  * Exponent bytes may be any: sums and maxima are kept so that neither very large
- * or small rows of V nor both beside each other leave the range of fp32 (rows of
- * one sequence and head whose exponents differ by more than 24 take longer).
+ * or small rows of V nor both beside each other leave the range of fp32 (where
+ * rows of V with bytes outside 80 .. 160 are seen, values under 1e-12 or over
+ * 1e12, the call takes several times as long).
  * Elements of q are held to 2^-25 (fp16) or 2^-21 (bf16) of their row's largest.
  * Weights p = exp(s) are rounded to 11 (fp16) or 8 (bf16) bits, with a floor of
  * 2^-21 or 2^-17 of the query's largest p_j * 2^e_j; one under 2^-126 of the
