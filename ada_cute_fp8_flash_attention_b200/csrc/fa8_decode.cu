@@ -374,6 +374,15 @@ __device__ __forceinline__ void wait_quietly(uint64_t* bar, uint32_t parity) {
   }
 }
 
+// The same for a copy that another role waits for and reports as well: until the
+// block gives up.
+__device__ __forceinline__ bool wait_along(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  const long long t0 = clock64();
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (*abort || clock64() - t0 > kTimeout) return false;
+  return true;
+}
+
 // ----------------------------------------------------------------------- work
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
   if (a.prefix_mode) return a.prefix_len;
@@ -653,7 +662,7 @@ __device__ __forceinline__ void floats_of(uint32_t w, float (&x)[4]) {
 
 // A block's share once more, by its softmax warps, in fp32 and straight from the
 // cache: for values so large or small that kRef does not serve them, or so far
-// apart. Four rows at a time; a warp takes every W-th run of 32
+// apart. R rows at a time; a warp takes every W-th run of 32
 // keys, a lane a key for the scores and D / 32 columns for the values. The
 // maximum of s is the weights' reference, that of s + e the sum of values', so
 // neither leaves the range of fp32. A call whose every share is computed again
@@ -662,7 +671,9 @@ __device__ __forceinline__ void floats_of(uint32_t w, float (&x)[4]) {
 // of it, with a second exponential for P, it cost every call 10 to 17 %.
 template <class C, bool kBf16>
 __device__ __forceinline__ void share_again(const Args& a, Walk walk, float* scratch) {
-  constexpr int D = C::D, W = C::NWG * 4, R = 4, V = D / 32;
+  // (Two rows in the blocks of which three share an SM: four spilled there, which
+  // the loop over tiles paid for as well.)
+  constexpr int D = C::D, W = C::NWG * 4, R = C::kCtas == 3 ? 2 : 4, V = D / 32;
   static_assert((R * D + 3 * W * R + W * R * D) * 4 <= C::kSlots * C::kSlotBytes, "scratch in the ring");
   float* const q_s = scratch;           // [R][D]
   float* const ms_s = q_s + R * D;      // [W][R] of each warp: maximum of s,
@@ -1344,9 +1355,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
           bool zero = false;
           const bool look = (first || up) && !dead && vb == kv::kExpBias;
           if (__any_sync(0xffffffffu, look)) {
+            // (The products wait for the tile too, and report one that fails to come.)
             const int st = (2 * n + 1) % NS;
-            ok = ok && wait.warp(&sh.kv_full[st], ((2 * n + 1) / NS) & 1);
-            if (look) zero = zero_row<D>(smem + st * C::kSlotBytes, tid);
+            if (wait_along(&sh.kv_full[st], ((2 * n + 1) / NS) & 1, &sh.abort) && look)
+              zero = zero_row<D>(smem + st * C::kSlotBytes, tid);
           }
           // (Zeros so far above the others that they set a maximum all the same.)
           if (zero) e1 = -kWide;
