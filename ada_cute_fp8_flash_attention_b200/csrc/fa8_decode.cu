@@ -65,18 +65,20 @@
 // waiting on the device for the first, joins them (always the same shares:
 // results repeat bit by bit).
 //
-// A shared prefix is one more set of items, whose rows are those of the whole
-// batch: one launch for it, one for what is behind it, one that joins both. A
-// prefix of few tiles is left in each sequence's own items (prefix_apart).
+// The whole pages of a shared prefix are one more set of items, whose rows are
+// those of the whole batch: one launch for it, one for what is behind it, one that
+// joins both. A prefix of few tiles is left in each sequence's own items
+// (prefix_apart).
 //
-// Measured on B200 (replayed from a graph, inputs in turn): 64 sequences of up
-// to 16384 keys, 32 heads on 8, bf16, 1.15 GB of cache: 176 us, 6.5 TB/s, the
-// measured copy rate. One sequence of 131072 keys, 32 heads on 4: 32 us, 4.2
-// TB/s: some 5 us until the first product and as many from the last to the
-// joined result are what a call costs that is this short. 64 sequences behind
-// 16384 shared keys: 86 us; there the chain of a tile (scores, maximum test,
-// exponentials, terms, values) in front of 64 rows bounds it, about 3000 clocks,
-// of which the exponentials take 512.
+// Measured on B200, inputs in turn: 64 sequences of up to 16384 keys, 32 heads on
+// 8, bf16, 1.15 GB of cache: 177 us replayed from a graph, 6.5 TB/s, the copy rate
+// measured beside it; 181 to 192 us called from Python one after another (over
+// boxes; 185 where the graph took 177), 6.0 to 6.3 TB/s. One sequence of 131072
+// keys, 32 heads on 4: 33 us replayed, 4.1 TB/s: some 5 us until the first product
+// and as many from the last to the joined result are what a call costs that is this
+// short. 64 sequences behind 16384 shared keys: 87 us; there the chain of a tile
+// (scores, maximum test, exponentials, terms, values) in front of 64 rows bounds
+// it, about 3000 clocks, of which the exponentials take 512.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
