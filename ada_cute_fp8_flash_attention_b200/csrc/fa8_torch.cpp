@@ -655,6 +655,8 @@ std::vector<torch::Tensor> flash_attn_fp8_decode(
                     out.sizes() == q.sizes() && out.is_non_overlapping_and_dense() && vec8_ok(out),
                 "out must be a dense tensor of q's shape and dtype, unit last stride, 16-byte "
                 "aligned");
+    // A query may be read again after a first result was written.
+    if (out.is_alias_of(q)) q = q.clone(at::MemoryFormat::Contiguous);
   } else {
     out = torch::empty({B, H, Sq, D}, q.options());
   }

@@ -364,7 +364,8 @@ int fa8_kv_read(const fa8_kv_copy_params* p, void* stream);
  * keys: query i of sequence b has position n = seqlens[b] - seqlen_q + i and
  * sees keys 0 .. n (its own K and V are in the cache already). q and o are
  * [batch][heads][seqlen_q][d] of type dtype (strides in elements, unit d;
- * those of q and o multiples of 8, bases 16-byte aligned); lse (optional) is
+ * those of q and o multiples of 8, bases 16-byte aligned; o may not overlap q); lse
+ * (optional) is
  * fp32 [batch][heads][seqlen_q], natural log, contiguous. Queries that see no
  * key give o = 0 and lse = -inf.
  *

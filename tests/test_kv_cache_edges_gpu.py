@@ -628,3 +628,23 @@ def test_extreme_queries_over_values_of_any_size(fa8, size, k_byte):
         want[0, 1] = want[1, 2] = True
         assert torch.equal(out.isnan().all(-1), want) and torch.equal(lse.isnan(), want)
         assert torch.equal(out[~want], got[0][~want])
+
+
+@pytest.mark.parametrize("prefix", [0, 1024])
+def test_result_over_its_own_queries(fa8, prefix):
+    """out=q, and out a view of q's memory, for ordinary values and for such as are
+    computed again."""
+    cache, table, seqlens, lens, q = prefix_case(fa8, 48, 32, 8, 1, 128, max(prefix, 64), 16, "bf16")
+    for far in (False, True):
+        if far:
+            cache.v_exp[:, :, ::5] += 60
+        call = lambda x, **kw: fa8.flash_attn_fp8_shared_prefix(  # noqa: E731
+            x, cache, table, seqlens, prefix, **kw)
+        want = call(q)
+        x = q.clone()
+        assert call(x, out=x).data_ptr() == x.data_ptr() and torch.equal(x, want)
+        room = torch.zeros(q.numel() + 4096, dtype=q.dtype, device="cuda")
+        x = room[:q.numel()].view(q.shape).copy_(q)
+        out = room[4096:].view(q.shape)
+        call(x, out=out)
+        assert torch.equal(out, want)
