@@ -159,7 +159,7 @@ struct Cfg {
   static constexpr int kCtas = resident(D, RW, NWG);
   // 227 KB a block, 228 KB an SM of which each block takes 1 KB and its
   // static variables; 1 KB to align.
-  static constexpr int kStatic = 2736 + 80 * kRows;
+  static constexpr int kStatic = 2736 + 80 * kRows + 16 * NWG;
   static constexpr int kBudget = (kCtas == 1 ? 227 : (228 - kCtas) / kCtas) * 1024 - kStatic - 1024;
   // P in two buffers where four tiles of the ring still fit beside them: the
   // next one is then written while the product of this one runs.
@@ -496,6 +496,8 @@ struct __align__(16) Shared {
     float step[C::RW];       // and what the last rise added to that
     float4 sum[C::RW];       // the four warps' sums of a row
     float4 top[C::RW];       // and maxima of a tile
+    uint32_t solid;          // a byte of each warp: has its part of the tile rows that are not zeros?
+    uint32_t pad[3];
   } g[C::NWG];
   static_assert(sizeof(Rows) % 16 == 0 && sizeof(Group) % 16 == 0, "read four at a time");
   static_assert(C::kSlots / 2 + 2 <= kExpTiles,
@@ -1270,8 +1272,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
 #pragma unroll
       for (int r = 0; r < RW / 2; ++r) l2[r] = 0;
       // Running maximum of row `lane`. A row that sees any of this block's keys
-      // of the item sees some of the first tile: that one sets it.
+      // of the item sees some of the first tile: that one sets it. As long as no
+      // value row but zeros has been met (`bare`) the next tile is looked at too.
       float m_lane = 0.f;
+      bool bare = true;
       if (lane < RW) g.neg_m[lane] = 0.f;  // (every warp writes the same)
       __syncwarp();
       for (int t = s.t0; t < s.t1; ++t, ++n) {
@@ -1342,7 +1346,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
         // Does a row rise above its maximum by more than kRise? Then the
         // largest s + e of each row over the tile is its new one.
         const bool up = high + e1 > kRise;
-        const bool rise = any_of(first || up || !ok);
+        const bool rise = any_of(bare || up || !ok);
         // An exponent that the reference does not serve.
         if (!dead && fabsf(e1) > kWide) sh.again = 1;
         // P's buffer is free: the product that read it two tiles ago was
@@ -1355,16 +1359,22 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
           // maximum of keys whose values are small, whose terms then vanish.
           // Looked at only where it could set a maximum.
           bool zero = false;
-          const bool look = (first || up) && !dead && vb == kv::kExpBias;
+          const bool look = (bare || up) && !dead && vb == kv::kExpBias;
           if (__any_sync(0xffffffffu, look)) {
             // (The products wait for the tile too, and report one that fails to come.)
             const int st = (2 * n + 1) % NS;
             if (wait_along(&sh.kv_full[st], ((2 * n + 1) / NS) & 1, &sh.abort) && look)
               zero = zero_row<D>(smem + st * C::kSlotBytes, tid);
           }
-          // (Zeros so far above the others that they set a maximum all the same.)
-          if (zero) e1 = -kWide;
+          // A maximum that zeros set all the same is kWide below their score. It is
+          // right unless values are met below it: beside them in a first tile, in
+          // the first tile with any behind tiles of zeros, or if it rises later.
+          if (zero) e1 = bare && !first ? -INFINITY : -kWide;
           if (zero && !first && high - kWide > kRise) sh.again = 1;
+          if (bare) {
+            const bool solid = __any_sync(0xffffffffu, !dead && !zero && !v_nan);
+            if (lane == 0) reinterpret_cast<uint8_t*>(&g.solid)[wq] = solid;
+          }
           float top = -INFINITY;
 #pragma unroll
           for (int r = 0; r < RW; r += 2) {
@@ -1382,10 +1392,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             left = true;
             break;
           }
+          const bool solid = g.solid != 0;
           float f_lane = 1.f;
           if (lane < RW) {
             const float4 v4 = g.top[lane];
             const float v = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
+            if (bare && !first && v < -1.f && v > -INFINITY) sh.again = 1;
             float by = 0.f;
             if (v > (first ? -INFINITY : kRise)) {
               by = v;
@@ -1404,7 +1416,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
               d2[r / 2 + 1] = ptx::fadd2(d2[r / 2 + 1], by.y);
             }
           }
-          if (first && __any_sync(0xffffffffu, zero)) {
+          if (first && solid && __any_sync(0xffffffffu, zero)) {
             float above = -INFINITY;
 #pragma unroll
             for (int r = 0; r < RW; r += 2) {
@@ -1416,6 +1428,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kCtas)
             }
             if (zero && above > kWide - 1.f) sh.again = 1;
           }
+          bare = !solid;
           if (t > s.t0) {
             // The sums so far, rescaled; O when the tile before is in it.
             const uint32_t rose = __ballot_sync(0xffffffffu, f_lane != 1.f);

@@ -648,3 +648,28 @@ def test_result_over_its_own_queries(fa8, prefix):
         out = room[4096:].view(q.shape)
         call(x, out=out)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("zeros", [128, 300, 1000])
+@pytest.mark.parametrize("keys", ["zeros", "ordinary"])
+@pytest.mark.parametrize("H,Hkv,Sq,D", [(8, 2, 1, 128), (16, 4, 3, 64), (40, 1, 1, 128)])
+def test_sequences_that_begin_with_zeros(fa8, H, Hkv, Sq, D, keys, zeros, dtype):
+    """Tokens whose values are zeros fill the first tiles: their own result is zero, and
+    what follows is as precise as without them."""
+    lens, ps = [zeros + 200, zeros, zeros + 3, zeros + 1500], 32
+    pages = pages_for(lens, ps)
+    cache = make_cache(fa8, pages, Hkv, ps, D, spread=0.3)
+    table, seqlens = make_table(lens, ps, pages)
+    for b in range(4):
+        for col in range(-(-zeros // ps)):
+            page, n = int(table[b, col]), min(ps, zeros - col * ps)
+            u8(cache.v)[page, :, :n] = 0
+            cache.v_exp[page, :, :n] = 127
+            if keys == "zeros":
+                u8(cache.k)[page, :, :n] = 0
+                cache.k_exp[page, :, :n] = 127
+    q = make_q(4, H, Sq, D, dtype)
+    got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+    assert bool((got[0][1] == 0).all()) and bool(torch.isfinite(got[1]).all())
+    assert_near(got, q, cache, table, lens)
