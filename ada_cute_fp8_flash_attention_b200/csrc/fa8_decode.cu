@@ -76,7 +76,7 @@
 // boxes; 185 where the graph took 177), 6.0 to 6.3 TB/s. One sequence of 131072
 // keys, 32 heads on 4: 33 us replayed, 4.1 TB/s: some 5 us until the first product
 // and as many from the last to the joined result are what a call costs that is this
-// short. 64 sequences behind 16384 shared keys: 87 us; there the chain of a tile
+// short. 64 sequences behind 16384 shared keys: 89 us; there the chain of a tile
 // (scores, maximum test, exponentials, terms, values) in front of 64 rows bounds
 // it, about 3000 clocks, of which the exponentials take 512.
 #include <cuda.h>
