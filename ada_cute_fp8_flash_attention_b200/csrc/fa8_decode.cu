@@ -85,6 +85,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -853,7 +854,10 @@ __device__ __forceinline__ void share_again(const Args& a, Walk walk, float* scr
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float out = x[v] * f0 * f1;
+          float out = x[v] * f0 * f1;
+          // A part that is to be weighted stays finite: bf16's largest is 2^128 as a
+          // code and a power of two, just above fp32's.
+          if (!(whole && a.own_rows) && fabsf(out) == INFINITY) out = copysignf(FLT_MAX, out);
           const int d = lane * V + v;
           if (!whole)
             a.part_o[at * D + d] = out;

@@ -376,8 +376,8 @@ int fa8_kv_read(const fa8_kv_copy_params* p, void* stream);
  * Elements of q are held to 2^-25 (fp16) or 2^-21 (bf16) of their row's largest.
  * Weights p = exp(s) are rounded to 11 (fp16) or 8 (bf16) bits, with a floor of
  * 2^-21 or 2^-17 of the query's largest p_j * 2^e_j; one under 2^-126 of the
- * query's largest may count as zero. A result beyond the type's range is
- * infinite.
+ * query's largest may count as zero, and a value beyond fp32's largest as that. A
+ * result beyond the type's range is infinite.
  *
  * prefix_len > 0: the first prefix_len tokens of all sequences are the same
  * (the caller vouches for it). Those in whole pages, the first prefix_len /

@@ -11,13 +11,15 @@ their sum, c_j the codes and 2^e_j the factor of value row j:
   sum B, and q's elements by half the least step of the last term: ds = D 2^-22 B +
   2^-21 (bf16) or 2^-25 (fp16) of the row's largest |q| times the largest scale *
   sum |k| of a key. It moves the quotient by 2 ds A. exp2 and sums: 2^-20 A; where
-  exponents of values differ by E, weights are exponentials of numbers up to E + 8
-  that were rounded twice: 2^-23 E A;
+  exponents of values differ by E, or are up to E (40 at most) away from -7, that of
+  unit normal rows, weights are exponentials of numbers up to E + 8 that were rounded
+  twice, each time by half a unit in the last place: ln 2 * 2^-23 (E + 8), of which 8
+  is within the 2^-20: 2^-23 E A;
 * results of parts are joined by their weights, and fp32 holds none under 2^-126
   of the row's largest (rounded up to a power of two): 2^-125 sum |v_j|;
 * small p meet a floor, 2^-17 or 2^-21 of the row's largest p_j 2^e_j over rows j
   that are not zero, for every key: that times sum_j |c_j| / w.
-lse: ds + 2^-20 (1 + |lse|). A result beyond the type's largest is infinite.
+lse: ds + 2^-23 E + 2^-20 (1 + |lse|). A result beyond the type's largest is infinite.
 """
 import math
 
@@ -80,16 +82,18 @@ def assert_near(got, q, cache, table, lens, scale=None):
             floor = lead[:, None] * c[:, :m].abs().sum(1) * 2.0 ** (-21 if fp16 else -17)
             E = (torch.where(solid, e[:, :m], -math.inf).amax(-1)
                  - torch.where(solid, e[:, :m], math.inf).amin(-1)).clamp(min=0).unsqueeze(-1)
+            away = torch.where(solid, (e[:, :m] + 7).abs(), 0.0).amax(-1).clamp(max=40)
+            E = torch.maximum(E, away.unsqueeze(-1))
             tol = ((u * want.abs()).clamp(min=least)
                    + (u + 2 * ds[:, None] + 2.0 ** -20 + 2.0 ** -23 * E) * A + floor
                    + 2.0 ** -125 * v[:, :m].abs().sum(1))
             err = (out[b, :, i].double() - want).abs()
-            far = want.abs() > top  # may round to the largest or to infinity
+            far = want.abs() + tol > top  # may be infinite
             bad = (~(err <= tol)) & ~far
             assert not bool(bad.any()), \
                 f"out: {float(err[bad].max()):.3g} over {float(tol[bad].min()):.3g}"
             wlse = torch.logsumexp(s, -1)
-            ltol = ds + 2.0 ** -20 * (1 + wlse.abs())
+            ltol = ds + 2.0 ** -23 * E.squeeze(-1) + 2.0 ** -20 * (1 + wlse.abs())
             lerr = (lse[b, :, i].double() - wlse).abs()
             assert bool((lerr <= ltol).all()), \
                 f"lse: {float(lerr.max()):.3g} over {float(ltol.min()):.3g}"
@@ -221,7 +225,9 @@ SIZES = {  # powers of two that value rows (of about 1) are multiplied by, by po
     "few large": lambda pos, rnd: torch.where(rnd > 0.99, 120.0, 0.0),
     "few small": lambda pos, rnd: torch.where(rnd > 0.99, -60.0, 20.0),
     "late": lambda pos, rnd: torch.where(pos > 0.97, 123.0, -30.0),
-    "near": lambda pos, rnd: 48 * rnd,  # about as far apart as one reference serves
+    "near": lambda pos, rnd: 48 * rnd,
+    "edges": lambda pos, rnd: torch.where(rnd > 0.5, 39.0, -39.0) + 3 * pos,  # of one reference
+    "low edge": lambda pos, rnd: -41 + 3 * rnd,
 }
 
 
@@ -673,3 +679,26 @@ def test_sequences_that_begin_with_zeros(fa8, H, Hkv, Sq, D, keys, zeros, dtype)
     got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
     assert bool((got[0][1] == 0).all()) and bool(torch.isfinite(got[1]).all())
     assert_near(got, q, cache, table, lens)
+
+
+def test_largest_value_of_bf16(fa8):
+    """bf16's largest rounds to 2^128 as a code and a factor, more than fp32 holds: keys
+    with such values count by their weights, whatever shares the work is cut into."""
+    D, H, Hkv, ps, n = 128, 8, 2, 16, 9000
+    top = torch.finfo(torch.bfloat16).max
+    pages = pages_for([n], ps)
+    cache = fa8.kv_cache_alloc(pages, Hkv, ps, D)
+    table, seqlens = make_table([n], ps, pages)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k = torch.randn(1, Hkv, n, D, generator=g, device="cuda")
+    v = torch.randn(1, Hkv, n, D, generator=g, device="cuda")
+    v[:, :, 100:300] = top
+    v[:, :, 5000:5010] = -top
+    v[:, 0, 8000] = top
+    fa8.kv_cache_write(cache, k.bfloat16(), v.bfloat16(), table, seqlens)
+    assert bool((cache.v.float()[cache.v_exp == 247].amax(-1) == 256).any())
+    for size in (0.1, 2.0):
+        q = make_q(1, H, 1, D, "bf16", size=size)
+        got = fa8.flash_attn_fp8_decode(q, cache, table, seqlens, return_lse=True)
+        assert not bool(got[0].isnan().any()) and not bool(got[0].isinf().any())
+        assert_near(got, q, cache, table, [n])
