@@ -10,11 +10,11 @@ their sum, c_j the codes and 2^e_j the factor of value row j:
 * scores: fp32 sums of D products, each addition off by 2^-22 of the largest partial
   sum B, and q's elements by half the least step of the last term: ds = D 2^-22 B +
   2^-21 (bf16) or 2^-25 (fp16) of the row's largest |q| times the largest scale *
-  sum |k| of a key. It moves the quotient by 2 ds A. exp2 and sums: 2^-20 A; where
+  sum |k| of a key. It moves the quotient by 2 ds A. exp2 and sums: 2^-20 A. Where
   exponents of values differ by E, or are up to E (40 at most) away from -7, that of
-  unit normal rows, weights are exponentials of numbers up to E + 8 that were rounded
-  twice, each time by half a unit in the last place: ln 2 * 2^-23 (E + 8), of which 8
-  is within the 2^-20: 2^-23 E A;
+  unit normal rows (rows of zeros count as 40 away), weights are exponentials of
+  numbers up to E + 8 that were rounded twice, each time by half a unit in the last
+  place: ln 2 * 2^-23 (E + 8), of which 8 is within the 2^-20: 2^-23 E A;
 * results of parts are joined by their weights, and fp32 holds none under 2^-126
   of the row's largest (rounded up to a power of two): 2^-125 sum |v_j|;
 * small p meet a floor, 2^-17 or 2^-21 of the row's largest p_j 2^e_j over rows j
@@ -82,7 +82,7 @@ def assert_near(got, q, cache, table, lens, scale=None):
             floor = lead[:, None] * c[:, :m].abs().sum(1) * 2.0 ** (-21 if fp16 else -17)
             E = (torch.where(solid, e[:, :m], -math.inf).amax(-1)
                  - torch.where(solid, e[:, :m], math.inf).amin(-1)).clamp(min=0).unsqueeze(-1)
-            away = torch.where(solid, (e[:, :m] + 7).abs(), 0.0).amax(-1).clamp(max=40)
+            away = torch.where(solid, (e[:, :m] + 7).abs(), 40.0).amax(-1).clamp(max=40)
             E = torch.maximum(E, away.unsqueeze(-1))
             tol = ((u * want.abs()).clamp(min=least)
                    + (u + 2 * ds[:, None] + 2.0 ** -20 + 2.0 ** -23 * E) * A + floor
